@@ -218,7 +218,7 @@ def _plain_select(st):
     x, scores, beam = st["logits"].double(), st["scores"].double(), st["case"]["beam"]
     B, K, V = x.shape
     top = x.amax(dim=-1, keepdim=True)
-    logp = x - (top + torch.log(torch.exp(x - top).sum(dim=-1, keepdim=True)))
+    logp = (x - top) - torch.log(torch.exp(x - top).sum(dim=-1, keepdim=True))
     if st["finished"] is not None:
         only = torch.full((V,), -math.inf, dtype=torch.float64, device=x.device)
         only[0] = 0.0
