@@ -24,6 +24,11 @@ from .linear import linear, pruned_joiner  # noqa: F401,E402
 from .rnnt_loss import get_rnnt_logprobs_pruned_joiner, rnnt_loss_pruned_joiner  # noqa: F401,E402
 from .mutual_information import provide_boundary_rows  # noqa: F401,E402
 
+# what stands on either side of the losses: the recurrence of the networks that make lm and am,
+# and the search that turns the trained joiner's logits into symbols
+from .recurrence import gated_recurrence, gated_recurrence_step  # noqa: F401,E402
+from .beam import beam_reorder, beam_select  # noqa: F401,E402
+
 
 def with_cuda() -> bool:
     """Counterpart of ``_fast_rnnt.with_cuda`` (always True here; raises if the

@@ -37,7 +37,8 @@ def lib():
                      "frnnt_simple_scratch_bytes", "frnnt_matmul_tn_scratch_floats",
                      "frnnt_joiner_input_grads_scratch_bytes", "frnnt_pruned_joiner_saved_bytes",
                      "frnnt_pruned_joiner_forward_scratch_bytes",
-                     "frnnt_pruned_joiner_backward_scratch_bytes"):
+                     "frnnt_pruned_joiner_backward_scratch_bytes",
+                     "frnnt_recurrence_saved_bytes"):
             if hasattr(_lib, name):
                 getattr(_lib, name).restype = _c_sz
     return _lib

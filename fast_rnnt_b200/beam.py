@@ -1,0 +1,99 @@
+"""Beam search on the GPU: the best continuations of every hypothesis by the trained joiner's
+logits, and the reordering of the hypotheses' states.  No counterpart in the reference, which
+ends with the losses.  The work runs in libfrnnt_sm100.so (csrc/beam.cu)."""
+from typing import List, Optional, Sequence, Tuple, Union
+
+import torch
+from torch import Tensor
+
+from . import _lib
+from ._lib import _c_int, _c_longlong, _c_vp
+
+
+def beam_select(logits: Tensor, scores: Tensor, beam: int, termination_symbol: int = 0,
+                finished: Optional[Tensor] = None) -> Tuple[Tensor, Tensor, Tensor]:
+    """The ``beam`` best continuations of every utterance: (scores, parents, tokens), each
+    [B][beam], best first.
+
+    logits [B][K][V] (float32, float16 or bfloat16, the vocabulary side by side, any strides
+    between rows) are the joiner's outputs for the K hypotheses of an utterance and scores
+    [B][K] (float32) their log-probabilities so far.  Hypothesis i goes on with symbol v at::
+
+        scores[b, i] + log_softmax(logits[b, i])[v]
+
+    and where ``finished`` (bool [B][K]) is set it only goes on with termination_symbol, at no
+    cost, its logits not read.  parents and tokens are int64: what continuation [b][j] goes on
+    from, and with what; equal scores go to the lower hypothesis and then to the lower symbol.
+
+    A hypothesis with a score of -inf or NaN is none (its logits are not read), a symbol whose
+    logit is -inf is never chosen, and a row whose log-sum-exp is not a finite number (a NaN or
+    +inf in it, or nothing but -inf) offers nothing.  Where fewer than ``beam`` continuations are
+    left, the slots behind them hold a score of -inf and -1 as parent and token, which
+    beam_reorder and gated_recurrence_step take as no hypothesis.
+
+    K is at most 1024, beam at most 32.  Not differentiable."""
+    assert logits.ndim == 3, logits.ndim
+    (B, K, V) = logits.shape
+    assert K >= 1 and V >= 1, logits.shape
+    assert scores.shape == (B, K), (scores.shape, logits.shape)
+    if logits.dtype != torch.float32 and not _lib.is_16bit(logits):
+        raise TypeError(f"only float32, float16 and bfloat16 logits are supported, got {logits.dtype}")
+    assert scores.dtype == torch.float32, scores.dtype
+    dev = logits.device
+    assert logits.is_cuda and scores.device == dev, (dev, scores.device)
+    if finished is not None:
+        assert finished.shape == (B, K) and finished.dtype == torch.bool, (finished.shape, finished.dtype)
+        assert finished.device == dev, (dev, finished.device)
+        assert 0 <= termination_symbol < V, (termination_symbol, V)
+        finished = finished.contiguous()
+    assert not (torch.is_grad_enabled() and (logits.requires_grad or scores.requires_grad)), \
+        "beam_select has no gradients: call it under torch.no_grad()"
+    if V > 1 and logits.stride(2) != 1:
+        logits = logits.contiguous()
+    scores = scores.contiguous()
+    with _lib.on_device(dev):
+        best = torch.empty(B, beam, dtype=torch.float32, device=dev)
+        parents = torch.empty(B, beam, dtype=torch.int64, device=dev)
+        tokens = torch.empty(B, beam, dtype=torch.int64, device=dev)
+        _lib.call("frnnt_beam_select", _c_int(_lib.input_code(logits.dtype)), _c_vp(logits.data_ptr()),
+                  _c_longlong(logits.stride(0)), _c_longlong(logits.stride(1)), _lib.ptr(scores),
+                  _lib.ptr(finished), int(termination_symbol), _lib.ptr(best), _lib.ptr(parents),
+                  _lib.ptr(tokens), B, K, V, int(beam), _lib.stream_ptr(dev))
+    return best, parents, tokens
+
+
+def beam_reorder(states: Union[Tensor, Sequence[Tensor]], parents: Tensor) -> Union[Tensor, List[Tensor]]:
+    """``states[b, parents[b, j]]`` for every tensor of ``states`` ([B][K][...], any types and
+    sizes), in one pass over all of them: new tensors [B][k][...], a list for a sequence of
+    tensors.  parents is int64 [B][k], as beam_select returns it; a parent outside 0 .. K-1 (-1:
+    no hypothesis) gives zeros.  Not differentiable."""
+    one = isinstance(states, Tensor)
+    tensors = [states] if one else list(states)
+    assert parents.ndim == 2 and parents.dtype == torch.int64, (parents.shape, parents.dtype)
+    (B, k) = parents.shape
+    dev = parents.device
+    assert parents.is_cuda, "fast_rnnt_b200 runs on CUDA tensors only (no CPU path)"
+    parents = parents.contiguous()
+    K = None
+    for t in tensors:
+        assert t.ndim >= 2 and t.shape[0] == B, (t.shape, parents.shape)
+        K = t.shape[1] if K is None else K
+        assert t.shape[1] == K and K >= 1, (t.shape, K)
+        assert t.device == dev, (t.device, dev)
+        assert not (torch.is_grad_enabled() and t.requires_grad), \
+            "beam_reorder has no gradients: call it under torch.no_grad()"
+    if not tensors:
+        return []
+    n = len(tensors)
+    with _lib.on_device(dev):
+        out = [torch.empty((B, k) + t.shape[2:], dtype=t.dtype, device=dev) for t in tensors]
+        # a row of a state has to lie in one piece; rows themselves may lie anywhere
+        flat = [t if t[0, 0].is_contiguous() else t.contiguous() for t in tensors] if B else tensors
+        size = [t.element_size() for t in flat]
+        row = [s * (t.numel() // (B * k) if B * k else 0) for s, t in zip(size, out)]
+        _lib.call("frnnt_beam_reorder", n, (_c_vp * n)(*[t.data_ptr() for t in flat]),
+                  (_c_longlong * n)(*[s * t.stride(0) for s, t in zip(size, flat)]),
+                  (_c_longlong * n)(*[s * t.stride(1) for s, t in zip(size, flat)]),
+                  (_c_vp * n)(*[t.data_ptr() for t in out]), (_c_longlong * n)(*row),
+                  _lib.ptr(parents), B, k, K, _lib.stream_ptr(dev))
+    return out[0] if one else out

@@ -417,6 +417,66 @@ int frnnt_pair_matmul_tn(const void *a_hi, const void *a_lo, const void *b_hi, c
                          const float *inv_scale_a, const float *inv_scale_b, float *d, float *partials,
                          int M, int N, long long R, long long pitch_a, long long pitch_b, void *stream);
 
+/* ----------------------------------------------------------------------------
+ * Gated linear recurrence (no counterpart in the reference)
+ * ------------------------------------------------------------------------- */
+
+/* For every channel d of every sequence b on its own, with f = 1 / (1 + exp(-gate)):
+ *   h[b][t][d] = f h[b][t-1][d] + (1 - f) x[b][t][d],   h[b][-1][d] = initial[b][d] (NULL: 0).
+ * dtype is FRNNT_F32, _F64, _F16 or _BF16, the type of x, gate and h (and of their gradients);
+ * initial, last and their gradients are float, double for FRNNT_F64, and so is all arithmetic.
+ * x and gate have D channels side by side and any strides, in elements, between batches and
+ * steps; h [B][T][D] and last [B][D] are contiguous and fully written.  lengths [B] (NULL: T
+ * everywhere) counts the steps of each sequence (below 0: 0, above T: T): the steps behind them
+ * are not read, h is zero there, and last is the state after the last step that counts.
+ * saved (NULL when no backward follows; frnnt_recurrence_saved_bytes) receives the states from
+ * which the backward recomputes h. */
+size_t frnnt_recurrence_saved_bytes(int dtype, int B, int T, int D);
+int frnnt_recurrence_forward(int dtype, const void *x, long long x_batch, long long x_step, const void *gate,
+                             long long gate_batch, long long gate_step, const void *initial,
+                             const int64_t *lengths, void *h, void *last, void *saved, int B, int T, int D,
+                             void *stream);
+
+/* Gradients of the above: dh (strided like x; NULL: zero) and dlast [B][D] (NULL: zero) give
+ * dx and dgate [B][T][D] and dinitial [B][D] (NULL: not wanted), fully written, zero behind
+ * the lengths. */
+int frnnt_recurrence_backward(int dtype, const void *x, long long x_batch, long long x_step, const void *gate,
+                              long long gate_batch, long long gate_step, const int64_t *lengths,
+                              const void *saved, const void *dh, long long dh_batch, long long dh_step,
+                              const void *dlast, void *dx, void *dgate, void *dinitial, int B, int T, int D,
+                              void *stream);
+
+/* One step of `rows` rows of D channels, x and gate with x_row / gate_row elements between rows:
+ * row r goes on from state[r], or with parents [rows] from state[(r / beams) * K + parents[r]]
+ * (zeros where the parent is not in 0 .. K-1).  next [rows][D] may not be state; h (NULL: not
+ * wanted) receives the new states in dtype. */
+int frnnt_recurrence_step(int dtype, const void *x, long long x_row, const void *gate, long long gate_row,
+                          const void *state, const int64_t *parents, void *h, void *next, long long rows,
+                          int beams, int K, int D, void *stream);
+
+/* ----------------------------------------------------------------------------
+ * Beam search (no counterpart in the reference)
+ * ------------------------------------------------------------------------- */
+
+/* The `beam` (1 to 32) best of the K * V continuations of each of B utterances, K at most 1024,
+ *   scores[b][i] + logits[b][i][v] - log(sum_v exp(logits[b][i][v])),
+ * in out_scores, out_parents (i) and out_tokens (v) [B][beam], best first, equal ones in the
+ * order of i * V + v.  dtype (FRNNT_F32, _F16, _BF16) is that of logits, whose rows hold V values
+ * side by side, `batch` / `row` elements apart.  finished [B][K] (bytes; NULL: none): a set byte
+ * leaves the row one continuation, `blank`, at its score.  A score of -inf or NaN, a logit of
+ * -inf and a row without a finite log-sum offer nothing; slots left over hold -inf, -1, -1. */
+int frnnt_beam_select(int dtype, const void *logits, long long batch, long long row, const float *scores,
+                      const uint8_t *finished, int blank, float *out_scores, int64_t *out_parents,
+                      int64_t *out_tokens, int B, int K, int V, int beam, void *stream);
+
+/* to[n][b][j] = from[n][b][parents[b][j]] for `count` tensors of rows of bytes[n] bytes, zeros
+ * where a parent is not in 0 .. K-1.  The five arrays are HOST arrays of `count` entries, read
+ * before the call returns; batch and beam are the strides of from[n] in bytes, to[n]
+ * [B][beams][bytes[n]] is contiguous and may not overlap from[n]. */
+int frnnt_beam_reorder(int count, const void *const *from, const long long *batch, const long long *beam,
+                       void *const *to, const long long *bytes, const int64_t *parents, int B, int beams,
+                       int K, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,240 @@
+"""beam_select and beam_reorder against their definitions in 64 bits."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+TYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+INF = math.inf
+
+
+def keys_of(logits, scores, finished=None, symbol=0):
+    """Every continuation's score in 64 bits, -inf where it is none."""
+    x, s = logits.detach().cpu().double(), scores.cpu().double()
+    top = x.amax(-1, keepdim=True)
+    logp = (x - top) - torch.log(torch.exp(x - top).sum(-1, keepdim=True))
+    if finished is not None:
+        f = finished.cpu()
+        logp[f] = -INF
+        logp[..., symbol] = torch.where(f, 0.0, logp[..., symbol])
+    key = s[:, :, None] + logp
+    return torch.where(torch.isnan(key), -INF, key).flatten(1)
+
+
+def tolerance(V):
+    """Of a score before its rounding to 32 bits: exponentials of 2^-21 relative error and no more
+    than V / 256 + 16 additions one after the other in 32 bits, each off by 2^-24 of the sum."""
+    return 2.0 ** -21 + (V / 256 + 16) * 2.0 ** -24
+
+
+def verify(logits, scores, beam, finished=None, symbol=0):
+    import fast_rnnt_b200 as fr
+    B, K, V = logits.shape
+    got, parents, tokens = fr.beam_select(logits, scores, beam, symbol, finished)
+    assert got.shape == parents.shape == tokens.shape == (B, beam)
+    key = keys_of(logits, scores, finished, symbol)
+    best, at = torch.sort(key, dim=1, descending=True, stable=True)
+    n = min(beam, K * V)
+    best, at = best[:, :n], at[:, :n]
+    got, parents, tokens = got.cpu(), parents.cpu(), tokens.cpu()
+    tol = tolerance(V)
+    for b in range(B):
+        m = int((best[b] > -INF).sum())
+        assert (got[b, m:] == -INF).all() and (parents[b, m:] == -1).all() and (tokens[b, m:] == -1).all(), b
+        p, t = parents[b, :m], tokens[b, :m]
+        assert ((p >= 0) & (p < K) & (t >= 0) & (t < V)).all(), (b, p, t)
+        index = p * V + t
+        assert len(set(index.tolist())) == m, (b, index)
+        off = (got[b, :m].double() - best[b, :m]).abs()
+        assert (off <= tol + 2.0 ** -24 * best[b, :m].abs()).all(), (b, off.max(), tol)
+        assert ((key[b, index] - best[b, :m]).abs() <= 2 * tol).all(), b
+        # the very continuation wherever its neighbours are further away than the tolerance, or
+        # equal to the last digit
+        for j in range(m):
+            near = (key[b] - best[b, j]).abs() <= 2 * tol
+            if not (near & (key[b] != best[b, j])).any():
+                assert index[j] == at[b, j], (b, j, index[j], at[b, j])
+    return got, parents, tokens
+
+
+def make(B, K, V, dtype, seed=0, scale=3.0):
+    g = torch.Generator().manual_seed(seed)
+    logits = (torch.randn(B, K, V, generator=g) * scale).to("cuda", TYPES[dtype])
+    return logits, (-8 * torch.rand(B, K, generator=g)).cuda()
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("B,K,V,beam", [(1, 1, 1, 1), (2, 1, 3, 8), (1, 4, 500, 4), (3, 4, 500, 10), (2, 3, 4233, 5),
+                                        (5, 16, 31, 16), (2, 8, 5000, 8), (1, 1, 50001, 32), (40, 5, 77, 3),
+                                        (3, 32, 1025, 32), (1, 3, 2049, 32), (2, 100, 40, 20), (600, 2, 130, 2)])
+def test_selection(B, K, V, beam, dtype):
+    logits, scores = make(B, K, V, dtype, seed=V)
+    verify(logits, scores, beam)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_dead_and_finished_hypotheses(dtype):
+    logits, scores = make(6, 7, 333, dtype, seed=1)
+    scores[0, 2:], scores[1, :], scores[2, 0], scores[2, 3] = -INF, -INF, float("nan"), -INF
+    logits[0, 3] = float("nan")             # not read: the hypothesis is none
+    finished = torch.zeros(6, 7, dtype=torch.bool)
+    finished[3], finished[4, ::2], finished[0, 0], finished[0, 3] = True, True, True, True
+    logits[4, 0] = float("nan")             # not read: the hypothesis is finished
+    verify(logits.masked_fill(torch.isnan(logits), 0.0), scores, 9, finished.cuda(), 17)
+    a = verify(logits.masked_fill(torch.isnan(logits), 0.0), scores, 9, finished.cuda())
+    import fast_rnnt_b200 as fr
+    b = fr.beam_select(logits, scores, 9, finished=finished.cuda())
+    assert all(torch.equal(u, v.cpu()) for u, v in zip(a, b))
+    assert (b[1][1] == -1).all() and (b[2][3, :7] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_masked_and_bad_logits(dtype):
+    logits, scores = make(7, 4, 700, dtype, seed=2)
+    logits[0, :, 5:] = -INF                  # few symbols allowed
+    logits[1, 1] = -INF                      # none
+    logits[2, 2, 11] = float("nan")          # the row offers nothing
+    logits[3, 0, 699] = INF
+    logits[4, :, 1:] = torch.finfo(TYPES[dtype]).min     # masked by the lowest number
+    logits[5] = torch.finfo(TYPES[dtype]).min
+    logits[6, :, :690] = -INF
+    verify(logits, scores, 12)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("V", [5, 64, 4233, 30000])
+def test_ties_go_to_the_lowest(V, dtype):
+    import fast_rnnt_b200 as fr
+    logits = torch.zeros(2, 3, V, dtype=TYPES[dtype], device="cuda")
+    logits[1] = 7
+    logits[1, :, 1::2] = 7.5
+    logits[0, :, 0] = -0.0
+    scores = torch.zeros(2, 3, device="cuda")
+    _, p, t = verify(logits, scores, min(32, V))
+    n = min(32, V)
+    assert (p[0] == 0).all() and torch.equal(t[0], torch.arange(n))
+    # equal hypotheses, wherever their rows lie
+    g = torch.Generator().manual_seed(3)
+    row = (torch.randn(V, generator=g) * 3).to("cuda", TYPES[dtype])
+    rows = row.expand(1, 9, V).contiguous()
+    s, p, t = fr.beam_select(rows, torch.zeros(1, 9, device="cuda"), 9)
+    assert torch.equal(p[0].cpu(), torch.arange(9)), p
+    assert (t == t[0, 0]).all() and (s == s[0, 0]).all()
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("V", [3000, 70001])
+def test_orders_that_come_in_clumps(V, dtype):
+    """Ascending, descending and periodic logits: the best ones lie side by side, or all in a few
+    threads' shares."""
+    n = torch.arange(V, dtype=torch.float64)
+    step = 8.0 / V
+    for x in (n * step, -n * step, torch.where(n % 2048 < 8, 5 + n * step, n * 0.0),
+              torch.where(n % 2048 < 256, (n % 7) * 0.5, n * 0.0), torch.where(n % 256 == 3, 4.0 + n % 3, n * 0.0)):
+        logits = x.to("cuda", TYPES[dtype])[None, None].repeat(2, 2, 1)
+        logits[1, 1] += 1
+        scores = torch.tensor([[0.0, -0.25], [-0.5, 0.0]], device="cuda")
+        verify(logits, scores, 32)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_strided_logits(dtype):
+    wide, scores = make(3, 5, 1001, dtype, seed=4)
+    verify(wide[:, :, :997], scores, 7)
+    verify(wide[:, :, 3:998], scores, 7)
+    verify(wide[:, ::2], scores[:, ::2], 7)
+    verify(wide.transpose(0, 1), scores.t(), 7)
+    verify(wide.transpose(1, 2)[:, :5], torch.zeros(3, 5, device="cuda"), 7)
+    verify(wide[:, :1].expand(3, 5, 1001), scores, 7)
+
+
+def test_select_offsets_beyond_32_bits():
+    V, K = 1 << 20, 9
+    logits = torch.zeros(240, K, V, dtype=torch.bfloat16, device="cuda")   # 2.2e9 elements
+    logits[-1] = make(1, K, V, "bf16", seed=5)[0][0]
+    scores = make(240, K, 4, "bf16", seed=6)[1]
+    import fast_rnnt_b200 as fr
+    got = fr.beam_select(logits, scores, 6)
+    want = fr.beam_select(logits[-1:].clone(), scores[-1:], 6)
+    assert all(torch.equal(a[-1:], b) for a, b in zip(got, want))
+    verify(logits[-1:], scores[-1:], 6)
+
+
+# ------------------------------------------------------------------------------
+def reordered(t, parents):
+    t, p = t.cpu(), parents.cpu()
+    B, K = t.shape[:2]
+    rows = torch.cat([t, torch.zeros_like(t[:, :1])], 1)
+    return rows[torch.arange(B)[:, None], torch.where((p < 0) | (p >= K), K, p)]
+
+
+@pytest.mark.parametrize("B,K,k", [(1, 1, 1), (3, 4, 4), (5, 2, 7), (2, 9, 1), (64, 8, 8)])
+def test_reorder(B, K, k):
+    import fast_rnnt_b200 as fr
+    g = torch.Generator().manual_seed(B)
+    parents = torch.randint(-1, K + 1, (B, k), generator=g).cuda()
+    states = [torch.randn(B, K, 37, generator=g).cuda(),
+              torch.randn(B, K, 512, generator=g).cuda().half(),
+              torch.randint(0, 9, (B, K, 65), generator=g).cuda(),
+              torch.randint(0, 2, (B, K), generator=g).bool().cuda(),
+              torch.randn(B, K, 3, 5, generator=g).cuda().bfloat16(),
+              torch.randn(B, K, 1, generator=g).cuda().double(),
+              torch.randn(B, K, 0, generator=g).cuda(),
+              torch.randn(B, K, 2, 64, generator=g).cuda()[:, :, 1],
+              torch.randn(K, B, 33, generator=g).cuda().transpose(0, 1),
+              torch.randn(B, K, 9, 4, generator=g).cuda().transpose(2, 3),
+              torch.randn(B, 1, 20, generator=g).cuda().expand(B, K, 20),
+              torch.randn(B, K, 5001, generator=g).cuda()[..., 1:]]
+    got = fr.beam_reorder(states, parents)
+    assert isinstance(got, list) and len(got) == len(states)
+    for t, u in zip(states, got):
+        assert u.dtype == t.dtype and torch.equal(u.cpu(), reordered(t, parents))
+    assert torch.equal(fr.beam_reorder(states[0], parents), got[0])
+    assert fr.beam_reorder([], parents) == []
+
+
+def test_reorder_many_and_large():
+    import fast_rnnt_b200 as fr
+    g = torch.Generator().manual_seed(7)
+    parents = torch.randint(-1, 3, (2, 5), generator=g).cuda()
+    states = [torch.randn(2, 3, 1 + 7 * n, generator=g).cuda() for n in range(70)]
+    for t, u in zip(states, fr.beam_reorder(tuple(states), parents)):
+        assert torch.equal(u.cpu(), reordered(t, parents))
+    # rows that begin beyond 2^31 elements
+    big = torch.zeros(2, 3, 400_000_001, dtype=torch.uint8, device="cuda")
+    big[1, 2, -1000:] = torch.arange(1000).cuda() % 251
+    out = fr.beam_reorder(big, torch.tensor([[0, 1], [1, 2]]).cuda())
+    assert torch.equal(out[1, 1], big[1, 2]) and not out[0].any() and not out[1, 0].any()
+
+
+def test_captured_search_step():
+    """Selection, reordering and the recurrence's step in one graph, replayed on other inputs."""
+    import fast_rnnt_b200 as fr
+
+    def step(logits, scores, states, x, gate, state):
+        with torch.no_grad():
+            best, parents, tokens = fr.beam_select(logits, scores, 4)
+            return (best, parents, tokens, *fr.beam_reorder(states, parents),
+                    *fr.gated_recurrence_step(x, gate, state, parents))
+
+    def inputs(seed):
+        logits, scores = make(3, 4, 500, "f32", seed=seed)
+        rest = [make(3, 4, n, "f32", seed=seed + n)[0] for n in (40, 7, 64, 64, 64)]
+        return [logits, scores, rest[:2], *rest[2:]]
+
+    static = inputs(1)
+    step(*static)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(*static)
+    for seed in (2, 1):
+        for s, t in zip(static, inputs(seed)):
+            for a, b in zip(s if isinstance(s, list) else [s], t if isinstance(t, list) else [t]):
+                a.copy_(b)
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(out, step(*inputs(seed))):
+            assert torch.equal(a, b)
