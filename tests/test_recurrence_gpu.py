@@ -45,7 +45,7 @@ def compare(got, want, names=None):
 
 
 SIZES = [(1, 1, 1), (2, 1, 7), (3, 2, 64), (2, 31, 33), (1, 32, 128), (2, 33, 8), (3, 127, 40), (2, 128, 72),
-         (2, 129, 65), (1, 257, 264), (2, 300, 24), (1, 1500, 16)]
+         (2, 129, 65), (1, 257, 264), (2, 300, 24), (1, 1500, 16), (2, 2500, 34), (1, 3000, 33)]
 
 
 @pytest.mark.parametrize("dtype", list(TYPES))
@@ -102,9 +102,12 @@ def test_gates_at_their_limits(dtype):
     x, gate, m = make(2, 300, 40, TYPES[dtype], seed=4)
     big = 60000.0
     gate[:, 10:20], gate[:, 30:35], gate[0, 40], gate[1, 41:260] = float("inf"), float("-inf"), -big, big
-    got = run(x, gate, **m)
-    compare(got, recurrence(x, gate, **m))
-    assert torch.equal(got["h"][:, 10:20], got["h"][:, 9:10].expand(-1, 10, -1))
+    got, want = run(x, gate, **m), recurrence(x, gate, **m)
+    compare(got, want)
+    # the state that a run of steps starts from is a product of gates times an earlier state, not
+    # the rounded chain, so that a kept state may differ between runs by its bound on either side
+    kept = (got["h"][:, 10:20] - got["h"][:, 9:10]).abs().cpu().double()
+    assert (kept <= want["h"][1][:, 10:20] + want["h"][1][:, 9:10]).all()
     assert torch.equal(got["h"][:, 30:35], x[:, 30:35])
     assert (got["dgate"][:, 10:20] == 0).all() and (got["dgate"][:, 30:35] == 0).all()
 
