@@ -23,9 +23,10 @@ def beam_select(logits: Tensor, scores: Tensor, beam: int, termination_symbol: i
 
     and where ``finished`` (bool [B][K]) is set it only goes on with termination_symbol, at no
     cost, its logits not read.  parents and tokens are int64: what continuation [b][j] goes on
-    from, and with what; equal scores go to the lower hypothesis and then to the lower symbol.
+    from, and with what.  Scores are compared in 64 bits and equal ones go to the lower
+    hypothesis; within a hypothesis the larger logit and then the lower symbol comes first.
 
-    A hypothesis with a score of -inf or NaN is none (its logits are not read), a symbol whose
+    A hypothesis with a score of -inf, +inf or NaN is none (its logits are not read), a symbol whose
     logit is -inf is never chosen, and a row whose log-sum-exp is not a finite number (a NaN or
     +inf in it, or nothing but -inf) offers nothing.  Where fewer than ``beam`` continuations are
     left, the slots behind them hold a score of -inf and -1 as parent and token, which

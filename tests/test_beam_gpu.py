@@ -88,6 +88,24 @@ def test_dead_and_finished_hypotheses(dtype):
     b = fr.beam_select(logits, scores, 9, finished=finished.cuda())
     assert all(torch.equal(u, v.cpu()) for u, v in zip(a, b))
     assert (b[1][1] == -1).all() and (b[2][3, :7] == 0).all()
+    # a score of +inf is as little a hypothesis as one of -inf
+    for value in (INF, -INF, float("nan")):
+        scores[5, 3] = value
+        got = fr.beam_select(logits, scores, 9)
+        assert (got[1][5] != 3).all() and torch.isfinite(got[0][5]).all()
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("K", range(1, 20))
+def test_every_number_of_hypotheses(K, dtype):
+    """Rows split over CTAs, one each, or several each: sizes on either side of every choice."""
+    for V in (1100, 2050, 17001):
+        logits, scores = make(2, K, V, dtype, seed=K)
+        scores[1, K // 2] = -INF
+        verify(logits, scores, 6)
+        finished = torch.zeros(2, K, dtype=torch.bool, device="cuda")
+        finished[:, -1] = True
+        verify(logits, scores, 6, finished, V - 1)
 
 
 @pytest.mark.parametrize("dtype", list(TYPES))
