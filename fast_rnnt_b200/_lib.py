@@ -38,7 +38,7 @@ def lib():
                      "frnnt_joiner_input_grads_scratch_bytes", "frnnt_pruned_joiner_saved_bytes",
                      "frnnt_pruned_joiner_forward_scratch_bytes",
                      "frnnt_pruned_joiner_backward_scratch_bytes",
-                     "frnnt_recurrence_saved_bytes"):
+                     "frnnt_recurrence_saved_bytes", "frnnt_beam_select_scratch_bytes"):
             if hasattr(_lib, name):
                 getattr(_lib, name).restype = _c_sz
     return _lib

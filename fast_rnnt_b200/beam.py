@@ -23,8 +23,8 @@ def beam_select(logits: Tensor, scores: Tensor, beam: int, termination_symbol: i
 
     and where ``finished`` (bool [B][K]) is set it only goes on with termination_symbol, at no
     cost, its logits not read.  parents and tokens are int64: what continuation [b][j] goes on
-    from, and with what.  Scores are compared in 64 bits and equal ones go to the lower
-    hypothesis; within a hypothesis the larger logit and then the lower symbol comes first.
+    from, and with what.  Scores are compared in 64 bits; equal ones go to the lower hypothesis
+    and then to the lower symbol.
 
     A hypothesis with a score of -inf, +inf or NaN is none (its logits are not read), a symbol whose
     logit is -inf is never chosen, and a row whose log-sum-exp is not a finite number (a NaN or
@@ -56,10 +56,13 @@ def beam_select(logits: Tensor, scores: Tensor, beam: int, termination_symbol: i
         best = torch.empty(B, beam, dtype=torch.float32, device=dev)
         parents = torch.empty(B, beam, dtype=torch.int64, device=dev)
         tokens = torch.empty(B, beam, dtype=torch.int64, device=dev)
-        _lib.call("frnnt_beam_select", _c_int(_lib.input_code(logits.dtype)), _c_vp(logits.data_ptr()),
+        code = _lib.input_code(logits.dtype)
+        scratch = torch.empty(max(_lib.size_of("frnnt_beam_select_scratch_bytes", code, B, K, V, beam), 1),
+                              dtype=torch.uint8, device=dev)
+        _lib.call("frnnt_beam_select", _c_int(code), _c_vp(logits.data_ptr()),
                   _c_longlong(logits.stride(0)), _c_longlong(logits.stride(1)), _lib.ptr(scores),
                   _lib.ptr(finished), int(termination_symbol), _lib.ptr(best), _lib.ptr(parents),
-                  _lib.ptr(tokens), B, K, V, int(beam), _lib.stream_ptr(dev))
+                  _lib.ptr(tokens), _lib.ptr(scratch), B, K, V, int(beam), _lib.stream_ptr(dev))
     return best, parents, tokens
 
 

@@ -1,27 +1,27 @@
 // Beam search: the best continuations over beams and vocabulary, and the reordering of states.
 //
-// beam_select, bound by one read of the logits.  A cluster of CTAs has an utterance; a CTA takes
-// whole rows (hypotheses) in turn, or one part of a row where there are fewer rows than CTAs.
+// beam_select, bound by one read of the logits, in two launches.  The first has a CTA for every
+// row (hypothesis), or for parts of rows where they are few, and leaves the `beam` best symbols
+// and the sum of exponentials of each; the second joins an utterance's rows.
 //
-//   stream   every thread reads 16 bytes at a time, keeping the running maximum and the sum of
-//            exponentials, and in which of its vectors the maximum lies: one pass gives the
-//            log-sum and, for every thread's share ("column"), its best symbol.
-//   columns  the `beam` threads with the largest maxima.  Whatever is among the best `beam` of the
-//            row lies in one of their columns: anything else is less than `beam` maxima.
-//   collect  those columns again (from L1 / L2, beam / 256 of the row), for all that is no less
-//            than the least of the chosen maxima: rarely more than `beam` and a few.
-//   order    by counting, for each, the greater ones.
+//   stream   every thread reads 16 bytes at a time and keeps the maximum and the sum of
+//            exponentials of its share ("column").
+//   bound    a logit that at least `beam` of the threads' maxima reach: the least, over the
+//            warps, of their m-th largest, with the warps' m making up `beam`.  Nothing below it
+//            is among the best `beam` of the row.
+//   collect  the columns whose maximum reaches the bound, again (from L1 / L2), for all that
+//            does: two to three times `beam` where logits are in no special order.
+//   order    by counting, for each, those before it.
 //
-// Lists of different rows are joined by the rank of each entry, which a binary search in the
-// other lists gives: no entry moves more than once, and there is no order in which atomics
-// could change the outcome.  Rows are read as vectors of the same elements wherever they begin
-// in memory (two aligned loads shifted into one off a 16-byte boundary), so that equal rows
-// have equal sums to the last bit and their ties are ties.
+// The second launch does the same with the entries of the rows' lists in place of logits.  Equal
+// logits of a row are in the order of their symbols and equal scores in that of i V + v, so that
+// no order of atomics could change the outcome.  Rows are read as vectors of the same elements
+// wherever they begin in memory (two aligned loads shifted into one off a 16-byte boundary), so
+// that equal rows have equal sums to the last bit and their ties are ties.
 //
-// Exponentials are the hardware's, in 32 bits relative to the maximum; the sums of the threads
-// are added, and scores kept and compared, in 64 bits.
-#include <cooperative_groups.h>
-
+// Exponentials are the hardware's, in 32 bits; the sums of a row's warps are added, and scores
+// computed and compared, in 64 bits.
+#include <cfloat>
 #include <climits>
 #include <type_traits>
 
@@ -33,12 +33,10 @@ constexpr int kSelThreads = 256;
 constexpr int kSelWarps = kSelThreads / 32;
 constexpr int kSelBeams = 1024;   // most rows of logits of one utterance
 constexpr int kSelMost = 32;      // most continuations
-constexpr int kSelCluster = 8;    // most CTAs of an utterance
-constexpr int kSelLists = 8;      // of rows, before they are joined; one per CTA of a cluster at the end
-constexpr int kSelBuffer = 1024;  // candidates of a row
-static_assert(kSelLists >= kSelCluster && kSelMost <= 32, "a list per CTA, a lane per entry");
+constexpr int kSelParts = 16;     // most parts of a row
+constexpr int kSelBuffer = 512;   // candidates, of a row or of an utterance's lists
 
-// order of floats as order of unsigned integers; the two zeros are one number
+// order of floating values as order of unsigned integers; the two zeros are one number
 __device__ __forceinline__ uint32_t ordered(float x) {
   const uint32_t u = __float_as_uint(x + 0.0f);
   return u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
@@ -53,12 +51,6 @@ __device__ __forceinline__ uint64_t ordered(double x) {
 __device__ __forceinline__ double unordered(uint64_t u) {
   return __longlong_as_double((long long)(u ^ ((uint64_t)((int64_t)~u >> 63) | 0x8000000000000000ull)));
 }
-// (value, place): larger values first, then lower places; 0 is less than any
-__device__ __forceinline__ uint64_t placed(float x, uint32_t place) {
-  return (uint64_t)ordered(x) << 32 | (0xffffffffu - place);
-}
-__device__ __forceinline__ uint32_t place_of(uint64_t p) { return 0xffffffffu - (uint32_t)p; }
-__device__ __forceinline__ float value_of(uint64_t p) { return unordered((uint32_t)(p >> 32)); }
 
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
@@ -69,353 +61,425 @@ __device__ __forceinline__ float exp2_fast(float x) {
 __device__ __forceinline__ float exp_below(float x, float top) {
   return exp2_fast((x - (top == neg_inf<float>() ? 0.0f : top)) * 1.4426950408889634f);
 }
+// log(x), x >= 1, off by 2^-26: the exponent's share in 64 bits, the rest below 0.35 in 32
+__device__ __forceinline__ double log_of(double x) {
+  const int e = (int)(((uint64_t)__double_as_longlong(x * 1.4142135623730951) >> 52) & 0x7ff) - 1023;
+  const double m = x * __longlong_as_double((long long)((uint64_t)(1023 - e) << 52));
+  const float f = (float)m;
+  return e * 0.6931471805599453 + (double)(logf(f) + (float)(m - (double)f) / f);
+}
 
 // ---- a row of logits as vectors of 16 bytes --------------------------------------------
+// Vector j holds elements EV j .. EV j + EV - 1 wherever the row begins; in memory it is the end
+// of one 16-byte granule and the beginning of the next (`off` elements on), or just a granule.
+// The granules of vectors 1 .. count - 3 lie within the row; the elements of the first and the
+// last two ("edges") are read one by one, a lane for each.
 template <typename T> struct SelRow {
   static constexpr int EV = 16 / (int)sizeof(T);
   const T *row;
-  int V, off, safe_lo, safe_hi;   // elements behind a 16-byte boundary; vectors that need no care
+  int V, off, half;   // off in elements; half: the bits of an odd 16-bit value's offset
   __device__ SelRow(const T *row_, int V_) : row(row_), V(V_) {
     off = (int)((uintptr_t)row % 16) / (int)sizeof(T);
-    safe_lo = off ? 1 : 0;
-    safe_hi = off ? (int)(((long long)V + off) / EV) - 1 : V / EV;
+    half = sizeof(T) == 2 && off % 2 ? 16 : 0;
   }
-  // vector j: elements EV j .. EV j + EV - 1, -inf behind the end
-  __device__ __forceinline__ uint4 load(int j) const {
-    if (j >= safe_lo && j < safe_hi) {
-      const uint4 *p = reinterpret_cast<const uint4 *>(row - off) + j;
-      const uint4 q = __ldg(p);
-      if (off == 0) return q;
+  __device__ __forceinline__ static int vectors(int V) { return (int)(((long long)V + EV - 1) / EV); }
+  // the symbol of a lane's edge element, -1: none
+  __device__ __forceinline__ int edge_symbol(int lane) const {
+    const long long v = lane < EV ? lane : (long long)max(1, vectors(V) - 2) * EV + lane - EV;
+    return lane < 3 * EV && v < V ? (int)v : -1;
+  }
+  // whole 32-bit words that the row begins behind a boundary; -1: on one
+  __device__ __forceinline__ int words() const { return off == 0 ? -1 : off * (int)sizeof(T) / 4; }
+  template <int W> __device__ __forceinline__ uint4 load(int j) const {
+    const uint4 *p = reinterpret_cast<const uint4 *>(row - off) + j;
+    const uint4 q = __ldg(p);
+    if constexpr (W < 0) {
+      return q;
+    } else {
       const uint4 r = __ldg(p + 1);
-      uint32_t w[8] = {q.x, q.y, q.z, q.w, r.x, r.y, r.z, r.w};
-      const int words = off * (int)sizeof(T) / 4;
-#pragma unroll
-      for (int n = 0; n < 7; ++n) w[n] = words & 1 ? w[n + 1] : w[n];
-#pragma unroll
-      for (int n = 0; n < 5; ++n) w[n] = words & 2 ? w[n + 2] : w[n];
-      if constexpr (sizeof(T) == 2) {
-        const int half = off & 1 ? 16 : 0;
-#pragma unroll
-        for (int n = 0; n < 4; ++n) w[n] = __funnelshift_r(w[n], w[n + 1], half);
-      }
-      return make_uint4(w[0], w[1], w[2], w[3]);
+      const uint32_t w[8] = {q.x, q.y, q.z, q.w, r.x, r.y, r.z, r.w};
+      if constexpr (sizeof(T) == 4) return make_uint4(w[W], w[W + 1], w[W + 2], w[W + 3]);
+      else
+        return make_uint4(__funnelshift_r(w[W], w[W + 1], half), __funnelshift_r(w[W + 1], w[W + 2], half),
+                          __funnelshift_r(w[W + 2], w[W + 3], half), __funnelshift_r(w[W + 3], w[(W + 4) % 8], half));
     }
-    T e[EV];
-#pragma unroll
-    for (int n = 0; n < EV; ++n) {
-      const long long v = (long long)j * EV + n;
-      e[n] = v < V ? row[v] : minus_inf();
-    }
-    uint4 q;
-    memcpy(&q, e, 16);
-    return q;
-  }
-  __device__ static __forceinline__ T minus_inf() {
-    if constexpr (sizeof(T) == 4) return -INFINITY;
-    else if constexpr (std::is_same<T, __half>::value) return __ushort_as_half(0xfc00);
-    else return __ushort_as_bfloat16(0xff80);
   }
   __device__ static __forceinline__ void unpack(const uint4 &q, float (&x)[EV]) {
-    T e[EV];
-    memcpy(e, &q, 16);
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
-    for (int n = 0; n < EV; ++n) x[n] = in_f32(e[n]);
+    for (int n = 0; n < 4; ++n) {
+      if constexpr (sizeof(T) == 4) {
+        x[n] = __uint_as_float(w[n]);
+      } else if constexpr (std::is_same<T, __half>::value) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[n]));
+        x[2 * n] = f.x, x[2 * n + 1] = f.y;
+      } else {
+        x[2 * n] = __uint_as_float(w[n] << 16), x[2 * n + 1] = __uint_as_float(w[n] & 0xffff0000u);
+      }
+    }
+  }
+  // the largest value that is a number
+  __device__ static __forceinline__ float most_of(const uint4 &q, const float (&x)[EV]) {
+    if constexpr (sizeof(T) == 4) {
+      return fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+    } else {
+      using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+      const T2 *h = reinterpret_cast<const T2 *>(&q);
+      const T2 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+      return fmaxf(in_f32(m.x), in_f32(m.y));
+    }
   }
 };
 
-// ---- lists of continuations, best first --------------------------------------------------
-struct SelEntry {
-  uint64_t key;     // ordered score
-  uint64_t symbol;  // (logit, symbol)
-  int row;
-};
-struct SelList {
-  uint64_t key[kSelMost], symbol[kSelMost];
-  int row[kSelMost], size;
-  __device__ __forceinline__ SelEntry get(int n) const { return {key[n], symbol[n], row[n]}; }
-  __device__ __forceinline__ void set(int n, const SelEntry &e) { key[n] = e.key, symbol[n] = e.symbol, row[n] = e.row; }
-};
-// Equal scores: the lower hypothesis; of one hypothesis the larger logit, then the lower symbol
-// (logits whose difference 64 bits of score do not show are in the order of the row's list too).
-__device__ __forceinline__ bool before(const SelEntry &a, const SelEntry &b) {
-  if (a.key != b.key) return a.key > b.key;
-  if (a.row != b.row) return a.row < b.row;
-  return a.symbol > b.symbol;
-}
-// how many entries of a list come before `e`
-__device__ __forceinline__ int rank_in(const SelList &list, const SelEntry &e) {
-  int lo = 0, hi = list.size;
-  while (lo < hi) {
-    const int mid = (lo + hi) / 2;
-    if (before(list.get(mid), e)) lo = mid + 1;
-    else hi = mid;
+// What a thread keeps of its share of a row.  Exponents are taken to base 2, x log2(e) - R in one
+// multiply-add with R = ref log2(e) rounded, and `ref` follows the maximum only when that is far
+// above it: nearly every vector raises some lane's maximum, hardly one needs the sums rescaled.
+// Beyond 1e38, where the product would overflow (rows masked by the lowest number there is), and
+// before the first number, it is exp(x - ref) the long way.
+struct SelShare {
+  float top = neg_inf<float>(), ref = neg_inf<float>(), R = 0;
+  float2 sum = {0, 0};
+  static constexpr float kLog2e = 1.4426950408889634f, kSlack = 20.0f;
+  __device__ static __forceinline__ bool plain(float x) { return fabsf(x) < 1e38f; }
+  __device__ __forceinline__ void rescale() {
+    const float by = plain(ref) ? exp2_fast(R - top * kLog2e) : exp_below(ref, top);
+    sum.x *= by;
+    sum.y *= by;
+    ref = top;
+    R = plain(top) ? top * kLog2e : 0.0f;
   }
-  return lo;
-}
-
-struct SelShared {
-  alignas(16) uint64_t buffer[kSelBuffer];
-  alignas(16) uint64_t lanes[kSelWarps][32];
-  uint64_t sorted[kSelWarps][32];
-  uint64_t top[kSelMost];
-  SelList lists[kSelLists], joined;
-  float part_top[kSelWarps];
-  double part_sum[kSelWarps];
-  float parts_top[kSelCluster];   // of a row in parts, from the CTAs of its parts
-  double parts_sum[kSelCluster];
-  float row_top;
-  double row_sum;
-  int found;
+  template <int EV> __device__ __forceinline__ void add(const float (&x)[EV], float most) {
+    top = fmaxf(top, most);
+    if (top > ref + kSlack) rescale();
+    if (plain(ref)) {
+      const float2 l = make_float2(kLog2e, kLog2e), r = make_float2(-R, -R);
+#pragma unroll
+      for (int e = 0; e < EV; e += 2) {
+        float2 t = __ffma2_rn(make_float2(x[e], x[e + 1]), l, r);
+        t.x = exp2_fast(t.x);
+        t.y = exp2_fast(t.y);
+        sum = __fadd2_rn(sum, t);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < EV; ++e) (e % 2 ? sum.y : sum.x) += exp_below(x[e], ref);
+    }
+  }
+  // sum of exp(x - top)
+  __device__ __forceinline__ float relative() const {
+    const float s = sum.x + sum.y;
+    return plain(ref) ? s * exp2f(-fmaf(top, kLog2e, -R)) : top > ref ? s * exp_below(ref, top) : s;
+  }
 };
 
-// lists[0 .. n-1] -> lists[0]
-__device__ void join_lists(SelShared &sm, int n, int beam) {
-  __syncthreads();
-  int total = 0;
-  for (int l = 0; l < n; ++l) total += sm.lists[l].size;
-  for (int e = threadIdx.x; e < n * beam; e += kSelThreads) {
-    const int l = e / beam, pos = e - l * beam;
-    if (pos >= sm.lists[l].size) continue;
-    const SelEntry own = sm.lists[l].get(pos);
-    int rank = pos;
-    for (int o = 0; o < n; ++o)
-      if (o != l) rank += rank_in(sm.lists[o], own);
-    if (rank < beam) sm.joined.set(rank, own);
-  }
-  __syncthreads();
-  const int size = total < beam ? total : beam;
-  if (threadIdx.x < size) sm.lists[0].set(threadIdx.x, sm.joined.get(threadIdx.x));
-  if (threadIdx.x == 0) sm.lists[0].size = size;
-  __syncthreads();
-}
-
-// The best `beam` symbols of vectors [first, end) of a row in sm.top, best first (0: none), and the
-// maximum and sum of exponentials in sm.row_top, sm.row_sum.
-template <typename T>
-__device__ void select_row(SelShared &sm, const SelRow<T> &row, int first, int end, int beam) {
+// W: see SelRow::words.  The loop's loads are under no branch but their predicate: with the edges
+// among them they would wait for one another (half the rate).
+template <typename T, int W>
+__device__ __forceinline__ void stream_row(SelShare &own, const SelRow<T> &row, int first, int end) {
   constexpr int EV = SelRow<T>::EV, U = 4;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  // stream
-  float top = neg_inf<float>(), sum = 0;
-  int top_at = 0;
-  for (int j0 = first + tid; j0 < end; j0 += U * kSelThreads) {
+  for (int j = first + (int)threadIdx.x; j < end; j += U * kSelThreads) {
     uint4 q[U];
 #pragma unroll
     for (int n = 0; n < U; ++n)
-      if (j0 + n * kSelThreads < end) q[n] = row.load(j0 + n * kSelThreads);
+      if (j + n * kSelThreads < end) q[n] = row.template load<W>(j + n * kSelThreads);
 #pragma unroll
-    for (int n = 0; n < U; ++n) {
-      const int j = j0 + n * kSelThreads;
-      if (j >= end) break;
-      float x[EV], most;
-      SelRow<T>::unpack(q[n], x);
-      most = x[0];
-#pragma unroll
-      for (int e = 1; e < EV; ++e) most = fmaxf(most, x[e]);
-      if (most > top) {
-        sum *= exp_below(top, most);
-        top = most;
-        top_at = j;
+    for (int n = 0; n < U; ++n)
+      if (j + n * kSelThreads < end) {
+        float x[EV];
+        SelRow<T>::unpack(q[n], x);
+        own.template add<EV>(x, SelRow<T>::most_of(q[n], x));
       }
-#pragma unroll
-      for (int e = 0; e < EV; ++e) sum += exp_below(x[e], top);
-    }
   }
-  // columns: in order within the warp, then among the warps
-  const uint64_t mine = top > neg_inf<float>() ? placed(top, (uint32_t)top_at) : 0;
-  sm.lanes[warp][lane] = mine;
-  sm.sorted[warp][lane] = 0;
-  if (tid < kSelMost) sm.top[tid] = 0;
-  if (tid == 0) sm.found = 0;
-  const float warp_top = warp_max(top);
-  const double warp_total = warp_sum((double)(sum * exp_below(top, warp_top)));
-  if (lane == 0) sm.part_top[warp] = warp_top, sm.part_sum[warp] = warp_total;
-  __syncwarp();
-  int rank = 0;
-#pragma unroll
-  for (int o = 0; o < 32; o += 2) {
-    const ulonglong2 two = *reinterpret_cast<const ulonglong2 *>(&sm.lanes[warp][o]);
-    rank += (two.x > mine) + (two.y > mine);
+}
+
+// An entry of a list: a logit and its symbol, larger logits first and then lower symbols; 0: none.
+__device__ __forceinline__ uint64_t entry_of(float x, uint32_t symbol) {
+  return (uint64_t)ordered(x) << 32 | (0xffffffffu - symbol);
+}
+__device__ __forceinline__ uint32_t symbol_of(uint64_t e) { return 0xffffffffu - (uint32_t)e; }
+__device__ __forceinline__ float logit_of(uint64_t e) { return unordered((uint32_t)(e >> 32)); }
+
+// The m-th largest of a warp's values (-inf where they are fewer), `each` = m.
+__device__ __forceinline__ float mth_of_warp(float own, int each) {
+  float most = own;
+  for (int n = 0; n < each; ++n) {
+    most = warp_max(own);
+    if ((threadIdx.x & 31) == __ffs(__ballot_sync(0xffffffffu, own == most)) - 1) own = neg_inf<float>();
   }
-  if (mine != 0) sm.sorted[warp][rank] = mine;
+  return most;
+}
+
+// What the first launch leaves of a row, or of a part of one; its list follows in `entries`.
+struct SelSum {
+  double sum;   // of exp(x - top)
+  float top;
+};
+
+struct RowShared {
+  uint64_t buffer[kSelBuffer], next[kSelWarps];
+  double part_sum[kSelWarps];
+  float part_top[kSelWarps], bound[kSelWarps];
+  int column[kSelThreads];
+  int found, columns;
+};
+
+template <typename T, int W>
+__device__ __forceinline__ void select_row(RowShared &sm, const SelRow<T> &row, int first, int end, bool edges,
+                                           SelSum *out, uint64_t *list, int beam) {
+  constexpr int EV = SelRow<T>::EV;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  // an edge element for the lanes of the last warp, which have least of the row to read
+  const int symbol = edges && warp == kSelWarps - 1 ? row.edge_symbol(lane) : -1;
+  const float edge = symbol >= 0 ? in_f32(row.row[symbol]) : neg_inf<float>();
+  SelShare own;
+  stream_row<T, W>(own, row, first, end);
+  const float column_top = own.top;
+  if (symbol >= 0) {
+    const float x[2] = {edge, neg_inf<float>()};
+    own.template add<2>(x, edge);
+  }
+  const float warp_top = warp_max(own.top);
+  const float warp_total = warp_sum(own.relative() * exp_below(own.top, warp_top));
+  // bound
+  const int whole = min(kSelWarps, max(1, (end - first) / 32));   // warps whose lanes all have a share
+  const float mth = mth_of_warp(own.top, (beam + whole - 1) / whole);
+  if (lane == 0) {
+    sm.part_top[warp] = warp_top;
+    sm.part_sum[warp] = warp_total;
+    sm.bound[warp] = warp < whole ? mth : INFINITY;
+  }
+  if (tid == 0) sm.found = sm.columns = 0;
+  if (tid < beam) list[tid] = 0;
   __syncthreads();
-  if (lane < beam && sm.sorted[warp][lane] != 0) {
-    const uint64_t key = sm.sorted[warp][lane];
-    int at[kSelWarps] = {};
+  float bound = INFINITY;
 #pragma unroll
-    for (int step = 16; step > 0; step >>= 1)
-#pragma unroll
-      for (int w = 0; w < kSelWarps; ++w)
-        if (sm.sorted[w][at[w] + step - 1] > key) at[w] += step;
-    int total = 0;
-#pragma unroll
-    for (int w = 0; w < kSelWarps; ++w) total += w == warp ? lane : at[w] + (at[w] == 31 && sm.sorted[w][31] > key);
-    if (total < beam) sm.top[total] = key;
+  for (int w = 0; w < kSelWarps; ++w) bound = fminf(bound, sm.bound[w]);
+  bound = fmaxf(bound, -FLT_MAX);   // -inf is no candidate
+  {
+    const bool chosen = column_top >= bound;
+    const unsigned all = __ballot_sync(0xffffffffu, chosen);
+    int slot = lane == 0 && all ? atomicAdd(&sm.columns, __popc(all)) : 0;
+    slot = __shfl_sync(0xffffffffu, slot, 0) + __popc(all & ((1u << lane) - 1));
+    if (chosen) sm.column[slot] = tid;
   }
-  if (warp == kSelWarps - 1 && lane < kSelWarps) {   // the row's maximum and sum
-    const unsigned mask = (1u << kSelWarps) - 1;
-    float m = sm.part_top[lane];
-    double s = sm.part_sum[lane];
+  if (tid == 0) {
+    float m = neg_inf<float>();
+    double sum = 0;
 #pragma unroll
-    for (int o = kSelWarps / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(mask, m, o));
-    s *= (double)exp_below(sm.part_top[lane], m);
+    for (int w = 0; w < kSelWarps; ++w) m = fmaxf(m, sm.part_top[w]);
 #pragma unroll
-    for (int o = kSelWarps / 2; o > 0; o >>= 1) s += __shfl_xor_sync(mask, s, o);
-    if (lane == 0) sm.row_top = m, sm.row_sum = s;
+    for (int w = 0; w < kSelWarps; ++w) sum += sm.part_sum[w] * (double)exp_below(sm.part_top[w], m);
+    out->top = m;
+    out->sum = sum;
   }
   __syncthreads();
   // collect
-  int columns = 0;
-  while (columns < beam && sm.top[columns] != 0) ++columns;
-  if (columns == 0) return;   // the whole CTA
-  // with fewer columns than `beam` there are no better ones elsewhere: all above -inf
-  const bool few = columns < beam;
-  const uint64_t least = sm.top[columns - 1];
-  const float least_value = few ? neg_inf<float>() : value_of(least);
-  const int least_at = few ? -1 : (int)place_of(least), deep = (end - first + kSelThreads - 1) / kSelThreads;
-  const auto each = [&](auto &&take) {
-    for (int p = tid; p < columns * deep; p += kSelThreads) {
-      const int c = p % columns;
-      const int j = first + ((int)place_of(sm.top[c]) - first) % kSelThreads + p / columns * kSelThreads;
+  const int pairs = sm.columns * ((end - first + kSelThreads - 1) / kSelThreads);
+  const auto collect = [&](auto &&take) {
+    if (edge >= bound) take(entry_of(edge, (uint32_t)symbol));
+    const int columns = sm.columns;
+    for (int p = tid; p < pairs; p += kSelThreads) {
+      const int level = p / columns, j = first + sm.column[p - level * columns] + level * kSelThreads;
       if (j >= end) continue;
+      const uint4 q = row.template load<W>(j);
       float x[EV];
-      SelRow<T>::unpack(row.load(j), x);
+      SelRow<T>::unpack(q, x);
+      if (!(SelRow<T>::most_of(q, x) >= bound)) continue;
 #pragma unroll
       for (int e = 0; e < EV; ++e)
-        if (x[e] > least_value || (x[e] == least_value && j <= least_at)) take(placed(x[e], (uint32_t)(j * EV + e)));
+        if (x[e] >= bound) take(entry_of(x[e], (uint32_t)(j * EV + e)));
     }
   };
-  each([&](uint64_t p) {
+  collect([&](uint64_t e) {
     const int n = atomicAdd(&sm.found, 1);
-    if (n < kSelBuffer) sm.buffer[n] = p;
+    if (n < kSelBuffer) sm.buffer[n] = e;
   });
   __syncthreads();
   const int found = sm.found;
   if (found <= kSelBuffer) {
-    // order
-    for (int c = tid; c < found; c += kSelThreads) {
-      const uint64_t own = sm.buffer[c];
-      int greater = 0;
-      for (int o = 0; o < found; ++o) greater += sm.buffer[o] > own;
-      if (greater < beam) sm.top[greater] = own;
+    // order: a warp for each
+    for (int c = warp; c < found; c += kSelWarps) {
+      const uint64_t mine = sm.buffer[c];
+      int earlier = 0;
+      for (int o = lane; o < found; o += 32) earlier += sm.buffer[o] > mine;
+      earlier = __reduce_add_sync(0xffffffffu, earlier);
+      if (lane == 0 && earlier < beam) list[earlier] = mine;
     }
   } else {
-    // more than the buffer holds, where the best ones lie in few columns: one at a time
-    uint64_t bound = ~0ull;
+    // more than the buffer holds (equal logits, or the best ones in few columns): one at a time
+    uint64_t last = ~0ull;
     for (int n = 0; n < beam; ++n) {
       uint64_t best = 0;
-      each([&](uint64_t p) { best = p < bound && p > best ? p : best; });
+      collect([&](uint64_t e) { best = e < last && e > best ? e : best; });
       for (int o = 16; o > 0; o >>= 1) {
         const uint64_t other = __shfl_xor_sync(0xffffffffu, best, o);
         best = other > best ? other : best;
       }
-      if (lane == 0) sm.lanes[0][warp] = best;
+      if (lane == 0) sm.next[warp] = best;
       __syncthreads();
-      for (int w = 0; w < kSelWarps; ++w) best = sm.lanes[0][w] > best ? sm.lanes[0][w] : best;
-      if (tid == 0) sm.buffer[n] = best;
-      bound = best;
+      for (int w = 0; w < kSelWarps; ++w) best = sm.next[w] > best ? sm.next[w] : best;
+      if (tid == 0) list[n] = best;
+      last = best;
       __syncthreads();
     }
-    if (tid < beam) sm.top[tid] = sm.buffer[tid];
   }
-  __syncthreads();
+}
+
+// a hypothesis: 0 none, 1 finished, 2 its row is read
+__device__ __forceinline__ int kind_of(float score, const uint8_t *finished, size_t at) {
+  return !(fabsf(score) < INFINITY) ? 0 : finished != nullptr && finished[at] != 0 ? 1 : 2;
 }
 
 template <typename T>
 __global__ void __launch_bounds__(kSelThreads, 4)
-beam_select_kernel(const T *__restrict__ logits, long long batch, long long row_stride,
+select_rows_kernel(const T *__restrict__ logits, long long batch, long long row_stride,
+                   const float *__restrict__ scores, const uint8_t *__restrict__ finished, int V,
+                   SelSum *__restrict__ sums, uint64_t *__restrict__ entries, int beam) {
+  __shared__ RowShared sm;
+  const int part = blockIdx.x, parts = gridDim.x, i = blockIdx.y, K = gridDim.y, b = blockIdx.z;
+  const size_t at = (size_t)b * K + i, unit = at * parts + part;
+  if (kind_of(scores[at], finished, at) != 2) return;
+  const int main_end = max(1, SelRow<T>::vectors(V) - 2), share = (main_end - 1 + parts - 1) / parts;
+  const int first = min(main_end, 1 + part * share), end = min(main_end, first + share);
+  const SelRow<T> row(logits + b * batch + i * row_stride, V);
+  SelSum *const sum = sums + unit;
+  uint64_t *const list = entries + unit * beam;
+  switch (row.words()) {
+    case -1: select_row<T, -1>(sm, row, first, end, part == 0, sum, list, beam); break;
+    case 0: select_row<T, 0>(sm, row, first, end, part == 0, sum, list, beam); break;
+    case 1: select_row<T, 1>(sm, row, first, end, part == 0, sum, list, beam); break;
+    case 2: select_row<T, 2>(sm, row, first, end, part == 0, sum, list, beam); break;
+    default: select_row<T, 3>(sm, row, first, end, part == 0, sum, list, beam); break;
+  }
+}
+
+// ---- joining an utterance's rows -------------------------------------------------------
+// A score as an ordered integer (0: none) and a place in K x V, lower places first.
+struct SelEntry {
+  uint64_t key;
+  uint32_t place;
+};
+__device__ __forceinline__ bool before(const SelEntry &a, const SelEntry &b) {
+  return a.key > b.key || (a.key == b.key && a.place < b.place);
+}
+
+__global__ void __launch_bounds__(kSelThreads)
+select_join_kernel(const SelSum *__restrict__ sums, const uint64_t *__restrict__ entries,
                    const float *__restrict__ scores, const uint8_t *__restrict__ finished, int blank,
                    float *__restrict__ out_scores, int64_t *__restrict__ out_parents,
                    int64_t *__restrict__ out_tokens, int K, int V, int parts, int beam) {
-  __shared__ SelShared sm;
-  namespace cg = cooperative_groups;
-  const int rank = blockIdx.x, ranks = gridDim.x, b = blockIdx.y, tid = threadIdx.x;
-  const int vectors = (int)(((long long)V + SelRow<T>::EV - 1) / SelRow<T>::EV);
-  const int share = (vectors + parts - 1) / parts;
-  if (parts > 1) {
-    if (tid < kSelCluster) sm.parts_top[tid] = neg_inf<float>(), sm.parts_sum[tid] = 0;
-    cg::this_cluster().sync();   // all have started, and have cleared theirs
+  __shared__ uint64_t key[kSelBuffer], next_key[kSelWarps];
+  __shared__ uint32_t place[kSelBuffer], next_place[kSelWarps];
+  __shared__ double row_log[kSelBeams];
+  __shared__ float row_top[kSelBeams], row_shift[kSelBeams];   // score less log-sum; -inf: offers nothing
+  __shared__ float warp_bound[kSelWarps], warp_widest[kSelWarps];
+  __shared__ int found;
+  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const SelSum *const sum = sums + (size_t)b * K * parts;
+  const uint64_t *const list = entries + (size_t)b * K * parts * beam;
+  // a row's log-sum.  A finished row is one whose only entry has logit and log-sum 0.
+  float widest = 0;
+  for (int i = tid; i < K; i += kSelThreads) {
+    const size_t at = (size_t)b * K + i;
+    const float score = scores[at];
+    const int kind = kind_of(score, finished, at);
+    float top = 0, shift = kind == 1 ? score : neg_inf<float>();
+    double log_sum = 0;
+    if (kind == 2) {
+      double total = 0;
+      top = neg_inf<float>();
+      for (int p = 0; p < parts; ++p) top = fmaxf(top, sum[i * parts + p].top);
+      for (int p = 0; p < parts; ++p)
+        total += sum[i * parts + p].sum * (double)exp_below(sum[i * parts + p].top, top);
+      log_sum = log_of(total);
+      if (fabsf(top) < INFINITY && total < (double)INFINITY)   // no NaN either
+        shift = (float)((double)score - (double)top - log_sum);
+    }
+    row_log[i] = log_sum;
+    row_top[i] = top;
+    row_shift[i] = shift;
+    if (shift != neg_inf<float>()) widest = fmaxf(widest, fabsf(shift));
   }
-  int lists = 0;
-  for (int unit = rank; unit < K * parts; unit += ranks) {
-    const int i = unit / parts, part = unit - i * parts;
-    const float score = scores[(size_t)b * K + i];
-    const bool none = !(fabsf(score) < INFINITY);
-    const bool done = !none && finished != nullptr && finished[(size_t)b * K + i] != 0;
-    const bool stream = !none && !done;
-    if (stream) {
-      const int first = part * share, end = min(vectors, first + share);
-      select_row<T>(sm, SelRow<T>(logits + b * batch + i * row_stride, V), first, end, beam);
-    }
-    if (parts > 1) {   // one unit per CTA: the parts of a row tell each other their sums
-      if (stream && tid < parts) {
-        SelShared *peer = cg::this_cluster().map_shared_rank(&sm, i * parts + tid);
-        peer->parts_top[part] = sm.row_top;
-        peer->parts_sum[part] = sm.row_sum;
-      }
-      cg::this_cluster().sync();
-      if (stream && tid == 0) {
-        float m = neg_inf<float>();
-        double s = 0;
-        for (int p = 0; p < parts; ++p) m = fmaxf(m, sm.parts_top[p]);
-        for (int p = 0; p < parts; ++p) s += sm.parts_sum[p] * (double)exp_below(sm.parts_top[p], m);
-        sm.row_top = m;
-        sm.row_sum = s;
-      }
-      __syncthreads();
-    }
-    SelList &list = sm.lists[lists];
-    if (stream) {
-      const float m = sm.row_top;
-      const bool fine = fabsf(m) < INFINITY && sm.row_sum < (double)INFINITY;   // no NaN either
-      if (tid < 32) {
-        const double log_sum = log(sm.row_sum);
-        const uint64_t symbol = tid < beam ? sm.top[tid] : 0;
-        const unsigned have = __ballot_sync(0xffffffffu, fine && symbol != 0);
-        if (symbol != 0)
-          list.set(tid, {ordered((double)score + (((double)value_of(symbol) - (double)m) - log_sum)), symbol, i});
-        if (tid == 0) list.size = __popc(have);
-      }
-      ++lists;
-    } else if (done && part == 0) {
-      if (tid == 0) {
-        list.set(0, {ordered((double)score), placed(0.0f, (uint32_t)blank), i});
-        list.size = 1;
-      }
-      ++lists;
-    }
-    if (lists == kSelLists) {
-      join_lists(sm, lists, beam);
-      lists = 1;
-    }
-    __syncthreads();
+  if (tid == 0) found = 0;
+  __syncthreads();
+  const int each_row = parts * beam;
+  const auto entry = [&](int n, int &i, bool &done) {   // the n-th of K x parts x beam; 0: none
+    i = n / each_row;
+    if (row_shift[i] == neg_inf<float>()) return (uint64_t)0;
+    done = finished != nullptr && finished[(size_t)b * K + i] != 0;
+    return !done ? list[n] : n == i * each_row ? entry_of(0.0f, (uint32_t)blank) : (uint64_t)0;
+  };
+  float best = neg_inf<float>();
+  for (int n = tid; n < K * each_row; n += kSelThreads) {
+    int i;
+    bool done;
+    const uint64_t e = entry(n, i, done);
+    if (e != 0) best = fmaxf(best, logit_of(e) + row_shift[i]);
   }
-  if (lists == 0) {
-    if (tid == 0) sm.lists[0].size = 0;
-    lists = 1;
-  }
-  if (lists > 1) join_lists(sm, lists, beam);
-  if (ranks > 1) {
-    cg::this_cluster().sync();
-    if (rank == 0) {
-      for (int e = tid; e < (ranks - 1) * beam; e += kSelThreads) {
-        const int l = 1 + e / beam, pos = e % beam;
-        const SelList &from = cg::this_cluster().map_shared_rank(&sm, l)->lists[0];
-        if (pos < from.size) sm.lists[l].set(pos, from.get(pos));
-        if (pos == 0) sm.lists[l].size = from.size;
-      }
+  const int whole = min(kSelWarps, max(1, K * each_row / 32));
+  const float mth = mth_of_warp(best, (beam + whole - 1) / whole);
+  widest = warp_max(widest);
+  if (lane == 0) warp_bound[warp] = warp < whole ? mth : INFINITY, warp_widest[warp] = widest;
+  __syncthreads();
+  float bound = INFINITY;
+#pragma unroll
+  for (int w = 0; w < kSelWarps; ++w) bound = fminf(bound, warp_bound[w]), widest = fmaxf(widest, warp_widest[w]);
+  // a score in 32 bits, logit + shift, is off by at most 2^-24 of itself and of the shift; beyond
+  // 1e30 (rows masked by the lowest numbers there are) all entries are taken
+  bound -= 4.0f * 0x1p-23f * (fabsf(bound) + widest);
+  if (!(widest < 1e30f)) bound = neg_inf<float>();
+  const auto collect = [&](auto &&take) {
+    for (int n = tid; n < K * each_row; n += kSelThreads) {
+      int i;
+      bool done;
+      const uint64_t e = entry(n, i, done);
+      if (e == 0 || logit_of(e) + row_shift[i] < bound) continue;
+      const double score = scores[(size_t)b * K + i];
+      const uint32_t v = symbol_of(e);
+      take(SelEntry{ordered(score + (((double)logit_of(e) - (double)row_top[i]) - row_log[i])), (uint32_t)i * (uint32_t)V + v});
     }
-    cg::this_cluster().sync();   // nobody reads another's lists any more
-    if (rank != 0) return;
-    join_lists(sm, ranks, beam);
-  }
-  if (tid < beam) {
-    const bool have = tid < sm.lists[0].size;
-    const SelEntry e = have ? sm.lists[0].get(tid) : SelEntry{};
+  };
+  collect([&](const SelEntry &e) {
+    const int n = atomicAdd(&found, 1);
+    if (n < kSelBuffer) key[n] = e.key, place[n] = e.place;
+  });
+  __syncthreads();
+  const auto write = [&](int n, const SelEntry &e) {
+    const size_t o = (size_t)b * beam + n;
+    out_scores[o] = (float)unordered(e.key);
+    out_parents[o] = (int64_t)(e.place / (uint32_t)V);
+    out_tokens[o] = (int64_t)(e.place % (uint32_t)V);
+  };
+  if (tid >= found && tid < beam) {   // slots left over
     const size_t o = (size_t)b * beam + tid;
-    out_scores[o] = have ? (float)unordered(e.key) : neg_inf<float>();
-    out_parents[o] = have ? e.row : -1;
-    out_tokens[o] = have ? (int64_t)place_of(e.symbol) : -1;
+    out_scores[o] = neg_inf<float>();
+    out_parents[o] = out_tokens[o] = -1;
+  }
+  if (found <= kSelBuffer) {
+    for (int c = warp; c < found; c += kSelWarps) {
+      const SelEntry mine = {key[c], place[c]};
+      int earlier = 0;
+      for (int o = lane; o < found; o += 32) earlier += before({key[o], place[o]}, mine);
+      earlier = __reduce_add_sync(0xffffffffu, earlier);
+      if (lane == 0 && earlier < beam) write(earlier, mine);
+    }
+    return;
+  }
+  SelEntry last = {~0ull, 0};
+  for (int n = 0; n < beam; ++n) {
+    SelEntry next = {0, 0xffffffffu};
+    collect([&](const SelEntry &e) { next = before(last, e) && before(e, next) ? e : next; });
+    for (int o = 16; o > 0; o >>= 1) {
+      const SelEntry other = {__shfl_xor_sync(0xffffffffu, next.key, o), __shfl_xor_sync(0xffffffffu, next.place, o)};
+      if (before(other, next)) next = other;
+    }
+    if (lane == 0) next_key[warp] = next.key, next_place[warp] = next.place;
+    __syncthreads();
+    for (int w = 0; w < kSelWarps; ++w)
+      if (before({next_key[w], next_place[w]}, next)) next = {next_key[w], next_place[w]};
+    if (tid == 0) write(n, next);
+    last = next;
+    __syncthreads();
   }
 }
 
@@ -452,27 +516,30 @@ beam_reorder_kernel(const __grid_constant__ ReorderList list, const int64_t *__r
   }
 }
 
-// Rows over the CTAs of a cluster: as many rows each as it takes for up to eight; with fewer
-// rows than that, rows in parts, each of two rounds of vectors or more.
+// Parts of a row: as many as give every multiprocessor two CTAs, each with two rounds of the
+// stream's loop or more.
+static int select_parts(int size, int B, int K, int V) {
+  const long long vectors = ((long long)V * size + 15) / 16;
+  int parts = 1;
+  while (parts < kSelParts && (long long)B * K * (parts + 1) <= 2 * sm_count() && (parts + 1) * 8 * kSelThreads <= vectors)
+    ++parts;
+  return parts;
+}
+
 template <typename T>
 static int select_launch(const T *logits, long long batch, long long row, const float *scores,
                          const uint8_t *finished, int blank, float *out_scores, int64_t *out_parents,
-                         int64_t *out_tokens, int B, int K, int V, int beam, cudaStream_t st) {
-  const int each = (K + kSelCluster - 1) / kSelCluster, vectors = (V + SelRow<T>::EV - 1) / SelRow<T>::EV;
-  int parts = 1, ranks = (K + each - 1) / each;
-  while (ranks + K <= kSelCluster && (parts + 1) * 2 * kSelThreads <= vectors) ++parts, ranks += K;
-  cudaLaunchConfig_t config = {};
-  config.gridDim = dim3((unsigned)ranks, (unsigned)B);
-  config.blockDim = dim3(kSelThreads);
-  config.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = (unsigned)ranks;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  config.attrs = attr;
-  config.numAttrs = ranks > 1 ? 1 : 0;
-  FRNNT_CUDA(FRNNT_KERNEL(cudaLaunchKernelEx(&config, beam_select_kernel<T>, logits, batch, row, scores, finished,
-                                             blank, out_scores, out_parents, out_tokens, K, V, parts, beam)));
+                         int64_t *out_tokens, void *scratch, int B, int K, int V, int beam, cudaStream_t st) {
+  const int parts = select_parts((int)sizeof(T), B, K, V);
+  SelSum *sums = (SelSum *)scratch;
+  uint64_t *entries = (uint64_t *)(sums + (size_t)B * K * parts);
+  FRNNT_KERNEL(select_rows_kernel<T><<<dim3((unsigned)parts, (unsigned)K, (unsigned)B), kSelThreads, 0, st>>>(
+      logits, batch, row, scores, finished, V, sums, entries, beam));
+  FRNNT_CUDA(cudaGetLastError());
+  FRNNT_KERNEL(select_join_kernel<<<(unsigned)B, kSelThreads, 0, st>>>(sums, entries, scores, finished, blank,
+                                                                       out_scores, out_parents, out_tokens, K, V,
+                                                                       parts, beam));
+  FRNNT_CUDA(cudaGetLastError());
   return FRNNT_OK;
 }
 
@@ -480,9 +547,14 @@ static int select_launch(const T *logits, long long batch, long long row, const 
 
 using namespace frnnt;
 
+extern "C" size_t frnnt_beam_select_scratch_bytes(int dtype, int B, int K, int V, int beam) {
+  if ((dtype != FRNNT_F32 && !is_half_input(dtype)) || B <= 0 || K <= 0 || V <= 0 || beam <= 0) return 0;
+  return (size_t)B * K * select_parts(is_half_input(dtype) ? 2 : 4, B, K, V) * (sizeof(SelSum) + beam * sizeof(uint64_t));
+}
+
 extern "C" int frnnt_beam_select(int dtype, const void *logits, long long batch, long long row, const float *scores,
                                  const uint8_t *finished, int blank, float *out_scores, int64_t *out_parents,
-                                 int64_t *out_tokens, int B, int K, int V, int beam, void *stream) {
+                                 int64_t *out_tokens, void *scratch, int B, int K, int V, int beam, void *stream) {
   FRNNT_REQUIRE(dtype == FRNNT_F32 || is_half_input(dtype), FRNNT_EINVAL, "dtype must be FRNNT_F32, _F16 or _BF16");
   FRNNT_REQUIRE(B >= 0 && K >= 1 && V >= 1, FRNNT_EINVAL, "bad sizes");
   FRNNT_REQUIRE(beam >= 1 && beam <= kSelMost, FRNNT_EUNSUPPORTED, "beam must be 1 to %d", kSelMost);
@@ -490,11 +562,12 @@ extern "C" int frnnt_beam_select(int dtype, const void *logits, long long batch,
   FRNNT_REQUIRE((long long)K * V < INT_MAX, FRNNT_EUNSUPPORTED, "beams times vocabulary must be below 2^31");
   FRNNT_REQUIRE(finished == nullptr || (blank >= 0 && blank < V), FRNNT_EINVAL, "termination symbol out of range");
   if (B == 0) return FRNNT_OK;
-  FRNNT_REQUIRE(logits && scores && out_scores && out_parents && out_tokens, FRNNT_EINVAL, "NULL argument");
+  FRNNT_REQUIRE(logits && scores && out_scores && out_parents && out_tokens && scratch, FRNNT_EINVAL, "NULL argument");
+  FRNNT_REQUIRE((uintptr_t)scratch % 16 == 0, FRNNT_EINVAL, "scratch must be 16-byte aligned");
   FRNNT_REQUIRE(B <= 65535, FRNNT_EUNSUPPORTED, "B too large for the grid");
 #define FRNNT_SELECT(TYPE)                                                                                \
   return select_launch<TYPE>((const TYPE *)logits, batch, row, scores, finished, blank, out_scores,       \
-                             out_parents, out_tokens, B, K, V, beam, (cudaStream_t)stream)
+                             out_parents, out_tokens, scratch, B, K, V, beam, (cudaStream_t)stream)
   if (dtype == FRNNT_F32) FRNNT_SELECT(float);
   if (dtype == FRNNT_F16) FRNNT_SELECT(__half);
   FRNNT_SELECT(__nv_bfloat16);

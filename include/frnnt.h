@@ -460,15 +460,16 @@ int frnnt_recurrence_step(int dtype, const void *x, long long x_row, const void 
 
 /* The `beam` (1 to 32) best of the K * V continuations of each of B utterances, K at most 1024,
  *   scores[b][i] + logits[b][i][v] - log(sum_v exp(logits[b][i][v])),
- * in out_scores, out_parents (i) and out_tokens (v) [B][beam], best first: of one row in the
- * order of the logits, equal ones in the order of v; of several rows in the order of the scores,
- * computed in 64 bits, equal ones in the order of i.  dtype (FRNNT_F32, _F16, _BF16) is that of logits, whose rows hold V values
+ * in out_scores, out_parents (i) and out_tokens (v) [B][beam], best first, compared in 64 bits,
+ * equal ones in the order of i * V + v.  dtype (FRNNT_F32, _F16, _BF16) is that of logits, whose rows hold V values
  * side by side, `batch` / `row` elements apart.  finished [B][K] (bytes; NULL: none): a set byte
  * leaves the row one continuation, `blank`, at its score.  A score of +-inf or NaN, a logit of
- * -inf and a row without a finite log-sum offer nothing; slots left over hold -inf, -1, -1. */
+ * -inf and a row without a finite log-sum offer nothing; slots left over hold -inf, -1, -1.
+ * scratch: frnnt_beam_select_scratch_bytes, 16-byte aligned. */
+size_t frnnt_beam_select_scratch_bytes(int dtype, int B, int K, int V, int beam);
 int frnnt_beam_select(int dtype, const void *logits, long long batch, long long row, const float *scores,
                       const uint8_t *finished, int blank, float *out_scores, int64_t *out_parents,
-                      int64_t *out_tokens, int B, int K, int V, int beam, void *stream);
+                      int64_t *out_tokens, void *scratch, int B, int K, int V, int beam, void *stream);
 
 /* to[n][b][j] = from[n][b][parents[b][j]] for `count` tensors of rows of bytes[n] bytes, zeros
  * where a parent is not in 0 .. K-1.  The five arrays are HOST arrays of `count` entries, read

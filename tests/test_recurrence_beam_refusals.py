@@ -72,7 +72,7 @@ def test_c_abi_checks(fr):
             text=b"overwrite")
     assert lib.frnnt_recurrence_saved_bytes(7, 1, 1, 1) == 0
     select = lambda dtype, B, K, V, beam, done=None, blank=0: (  # noqa: E731
-        "frnnt_beam_select", dtype, one, n(V), n(V), one, done, blank, one, one, one, B, K, V, beam, None)
+        "frnnt_beam_select", dtype, one, n(V), n(V), one, done, blank, one, one, one, one, B, K, V, beam, None)
     refused(*select(1, 1, 2, 5, 2), text=b"dtype")
     refused(*select(0, 1, 0, 5, 2), text=b"sizes")
     refused(*select(0, 1, 2, 5, 0), code=-2, text=b"beam")
