@@ -20,6 +20,18 @@ _c_int, _c_vp, _c_sz, _c_f64 = ctypes.c_int, ctypes.c_void_p, ctypes.c_size_t, c
 _c_longlong = ctypes.c_longlong
 
 
+# Arguments of the calls that decoding makes per symbol, where a converter looked up once costs
+# less than an object made per argument: p pointer (an integer or None), l 64 bits, i int.
+_KINDS = {"p": _c_vp, "l": _c_longlong, "i": ctypes.c_int}
+_ARGUMENTS = {
+    "frnnt_recurrence_forward": "ipllpllpppppiiip",
+    "frnnt_recurrence_backward": "ipllpllpppllppppiiip",
+    "frnnt_recurrence_step": "iplplppppliiip",
+    "frnnt_beam_select": "ipllppippppiiiip",
+    "frnnt_beam_reorder": "ipppppp" + "iiip",
+}
+
+
 class FrnntError(RuntimeError):
     pass
 
@@ -41,6 +53,8 @@ def lib():
                      "frnnt_recurrence_saved_bytes", "frnnt_beam_select_scratch_bytes"):
             if hasattr(_lib, name):
                 getattr(_lib, name).restype = _c_sz
+        for name, kinds in _ARGUMENTS.items():
+            getattr(_lib, name).argtypes = [_KINDS[k] for k in kinds]
     return _lib
 
 

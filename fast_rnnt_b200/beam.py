@@ -1,13 +1,14 @@
 """Beam search on the GPU: the best continuations of every hypothesis by the trained joiner's
 logits, and the reordering of the hypotheses' states.  No counterpart in the reference, which
 ends with the losses.  The work runs in libfrnnt_sm100.so (csrc/beam.cu)."""
+import math
 from typing import List, Optional, Sequence, Tuple, Union
 
 import torch
 from torch import Tensor
 
 from . import _lib
-from ._lib import _c_int, _c_longlong, _c_vp
+from ._lib import _c_longlong, _c_vp
 
 
 def beam_select(logits: Tensor, scores: Tensor, beam: int, termination_symbol: int = 0,
@@ -52,17 +53,17 @@ def beam_select(logits: Tensor, scores: Tensor, beam: int, termination_symbol: i
     if V > 1 and logits.stride(2) != 1:
         logits = logits.contiguous()
     scores = scores.contiguous()
+    code, (sb, sk, _) = _lib.input_code(logits.dtype), logits.stride()
     with _lib.on_device(dev):
-        best = torch.empty(B, beam, dtype=torch.float32, device=dev)
-        parents = torch.empty(B, beam, dtype=torch.int64, device=dev)
-        tokens = torch.empty(B, beam, dtype=torch.int64, device=dev)
-        code = _lib.input_code(logits.dtype)
-        scratch = torch.empty(max(_lib.size_of("frnnt_beam_select_scratch_bytes", code, B, K, V, beam), 1),
-                              dtype=torch.uint8, device=dev)
-        _lib.call("frnnt_beam_select", _c_int(code), _c_vp(logits.data_ptr()),
-                  _c_longlong(logits.stride(0)), _c_longlong(logits.stride(1)), _lib.ptr(scores),
-                  _lib.ptr(finished), int(termination_symbol), _lib.ptr(best), _lib.ptr(parents),
-                  _lib.ptr(tokens), _lib.ptr(scratch), B, K, V, int(beam), _lib.stream_ptr(dev))
+        best = scores.new_empty((B, beam))
+        parents = scores.new_empty((B, beam), dtype=torch.int64)
+        tokens = torch.empty_like(parents)
+        n = _lib.size_of("frnnt_beam_select_scratch_bytes", code, B, K, V, beam)
+        scratch = scores.new_empty(n, dtype=torch.uint8)
+        _lib.call("frnnt_beam_select", code, logits.data_ptr(), sb, sk, scores.data_ptr(),
+                  None if finished is None else finished.data_ptr(), termination_symbol,
+                  best.data_ptr(), parents.data_ptr(), tokens.data_ptr(), scratch.data_ptr(), B, K, V,
+                  beam, _lib.stream_ptr(dev))
     return best, parents, tokens
 
 
@@ -78,26 +79,33 @@ def beam_reorder(states: Union[Tensor, Sequence[Tensor]], parents: Tensor) -> Un
     dev = parents.device
     assert parents.is_cuda, "fast_rnnt_b200 runs on CUDA tensors only (no CPU path)"
     parents = parents.contiguous()
-    K = None
-    for t in tensors:
-        assert t.ndim >= 2 and t.shape[0] == B, (t.shape, parents.shape)
-        K = t.shape[1] if K is None else K
-        assert t.shape[1] == K and K >= 1, (t.shape, K)
-        assert t.device == dev, (t.device, dev)
-        assert not (torch.is_grad_enabled() and t.requires_grad), \
-            "beam_reorder has no gradients: call it under torch.no_grad()"
     if not tensors:
         return []
-    n = len(tensors)
+    K, grad = None, torch.is_grad_enabled()
+    start, pitch, step, row = [], [], [], []
     with _lib.on_device(dev):
-        out = [torch.empty((B, k) + t.shape[2:], dtype=t.dtype, device=dev) for t in tensors]
-        # a row of a state has to lie in one piece; rows themselves may lie anywhere
-        flat = [t if t[0, 0].is_contiguous() else t.contiguous() for t in tensors] if B else tensors
-        size = [t.element_size() for t in flat]
-        row = [s * (t.numel() // (B * k) if B * k else 0) for s, t in zip(size, out)]
-        _lib.call("frnnt_beam_reorder", n, (_c_vp * n)(*[t.data_ptr() for t in flat]),
-                  (_c_longlong * n)(*[s * t.stride(0) for s, t in zip(size, flat)]),
-                  (_c_longlong * n)(*[s * t.stride(1) for s, t in zip(size, flat)]),
-                  (_c_vp * n)(*[t.data_ptr() for t in out]), (_c_longlong * n)(*row),
-                  _lib.ptr(parents), B, k, K, _lib.stream_ptr(dev))
+        out = []
+        for n, t in enumerate(tensors):
+            shape = t.shape
+            assert len(shape) >= 2 and shape[0] == B, (shape, parents.shape)
+            K = shape[1] if n == 0 else K
+            assert shape[1] == K and K >= 1, (shape, K)
+            assert t.device == dev, (t.device, dev)
+            assert not (grad and t.requires_grad), \
+                "beam_reorder has no gradients: call it under torch.no_grad()"
+            # a row of a state has to lie in one piece; rows themselves may lie anywhere
+            if not t.is_contiguous() and B > 0 and not t[0, 0].is_contiguous():
+                t = tensors[n] = t.contiguous()
+            size, stride = t.element_size(), t.stride()
+            out.append(torch.empty_like(t, memory_format=torch.contiguous_format) if k == K
+                       else t.new_empty((B, k) + shape[2:]))
+            start.append(t.data_ptr())
+            pitch.append(size * stride[0])
+            step.append(size * stride[1])
+            row.append(size * math.prod(shape[2:]))
+        n = len(tensors)
+        words, pointers = _c_longlong * n, _c_vp * n
+        _lib.call("frnnt_beam_reorder", n, pointers(*start), words(*pitch), words(*step),
+                  pointers(*[t.data_ptr() for t in out]), words(*row), parents.data_ptr(), B, k, K,
+                  _lib.stream_ptr(dev))
     return out[0] if one else out

@@ -4,13 +4,14 @@
 // row (hypothesis), or for parts of rows where they are few, and leaves the `beam` best symbols
 // and the sum of exponentials of each; the second joins an utterance's rows.
 //
-//   stream   every thread reads 16 bytes at a time and keeps the maximum and the sum of
-//            exponentials of its share ("column").
+//   stream   every thread reads 16 bytes at a time and keeps the sum of exponentials of its
+//            share ("column"), the maximum, which vector holds it, and the next vector's maximum.
 //   bound    a logit that at least `beam` of the threads' maxima reach: the least, over the
 //            warps, of their m-th largest, with the warps' m making up `beam`.  Nothing below it
 //            is among the best `beam` of the row.
-//   collect  the columns whose maximum reaches the bound, again (from L1 / L2), for all that
-//            does: two to three times `beam` where logits are in no special order.
+//   collect  the vectors whose maximum reaches the bound, again (from L1 / L2), for all that
+//            does: two to three times `beam` where logits are in no special order.  Of a column
+//            whose next maximum reaches it too, all vectors are looked at.
 //   order    by counting, for each, those before it.
 //
 // The second launch does the same with the entries of the rows' lists in place of logits.  Equal
@@ -29,7 +30,9 @@
 
 namespace frnnt {
 
-constexpr int kSelThreads = 256;
+// Small CTAs, many of them: a row's short phases after the stream run beside other rows' streams
+// (96 x 16 x 31999 fp16: 35 us; 256 threads, 5 CTAs a multiprocessor 39; 64 threads, 24 CTAs 48).
+constexpr int kSelThreads = 128, kSelResident = 12;
 constexpr int kSelWarps = kSelThreads / 32;
 constexpr int kSelBeams = 1024;   // most rows of logits of one utterance
 constexpr int kSelMost = 32;      // most continuations
@@ -131,14 +134,34 @@ template <typename T> struct SelRow {
   }
 };
 
+// vector j, the shift at run time (the collection's few vectors: one copy of that code)
+template <typename T> __device__ __forceinline__ uint4 load_any(const SelRow<T> &row, int j) {
+  const uint4 *p = reinterpret_cast<const uint4 *>(row.row - row.off) + j;
+  const uint4 q = __ldg(p);
+  if (row.off == 0) return q;
+  const uint4 r = __ldg(p + 1);
+  uint32_t w[8] = {q.x, q.y, q.z, q.w, r.x, r.y, r.z, r.w};
+  const int words = row.words();
+#pragma unroll
+  for (int n = 0; n < 7; ++n) w[n] = words & 1 ? w[n + 1] : w[n];
+#pragma unroll
+  for (int n = 0; n < 5; ++n) w[n] = words & 2 ? w[n + 2] : w[n];
+  if constexpr (sizeof(T) == 2) {
+#pragma unroll
+    for (int n = 0; n < 4; ++n) w[n] = __funnelshift_r(w[n], w[n + 1], row.half);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
 // What a thread keeps of its share of a row.  Exponents are taken to base 2, x log2(e) - R in one
 // multiply-add with R = ref log2(e) rounded, and `ref` follows the maximum only when that is far
 // above it: nearly every vector raises some lane's maximum, hardly one needs the sums rescaled.
 // Beyond 1e38, where the product would overflow (rows masked by the lowest number there is), and
 // before the first number, it is exp(x - ref) the long way.
 struct SelShare {
-  float top = neg_inf<float>(), ref = neg_inf<float>(), R = 0;
+  float top = neg_inf<float>(), next = neg_inf<float>(), ref = neg_inf<float>(), R = 0;
   float2 sum = {0, 0};
+  int at = 0;   // the vector of `top`; `next` is the maximum of the others
   static constexpr float kLog2e = 1.4426950408889634f, kSlack = 20.0f;
   __device__ static __forceinline__ bool plain(float x) { return fabsf(x) < 1e38f; }
   __device__ __forceinline__ void rescale() {
@@ -148,8 +171,9 @@ struct SelShare {
     ref = top;
     R = plain(top) ? top * kLog2e : 0.0f;
   }
-  template <int EV> __device__ __forceinline__ void add(const float (&x)[EV], float most) {
-    top = fmaxf(top, most);
+  template <int EV> __device__ __forceinline__ void add(const float (&x)[EV], float most, int j) {
+    next = fmaxf(next, fminf(top, most));
+    if (most > top) top = most, at = j;
     if (top > ref + kSlack) rescale();
     if (plain(ref)) {
       const float2 l = make_float2(kLog2e, kLog2e), r = make_float2(-R, -R);
@@ -173,21 +197,23 @@ struct SelShare {
 };
 
 // W: see SelRow::words.  The loop's loads are under no branch but their predicate: with the edges
-// among them they would wait for one another (half the rate).
+// among them they would wait for one another (half the rate).  A row that is not to be read is
+// left when the first loads are under way: they do not wait for the scores.
 template <typename T, int W>
-__device__ __forceinline__ void stream_row(SelShare &own, const SelRow<T> &row, int first, int end) {
-  constexpr int EV = SelRow<T>::EV, U = 4;
+__device__ __forceinline__ void stream_row(SelShare &own, const SelRow<T> &row, int first, int end, bool read) {
+  constexpr int EV = SelRow<T>::EV, U = 2;
   for (int j = first + (int)threadIdx.x; j < end; j += U * kSelThreads) {
     uint4 q[U];
 #pragma unroll
     for (int n = 0; n < U; ++n)
       if (j + n * kSelThreads < end) q[n] = row.template load<W>(j + n * kSelThreads);
+    if (!read) return;
 #pragma unroll
     for (int n = 0; n < U; ++n)
       if (j + n * kSelThreads < end) {
         float x[EV];
         SelRow<T>::unpack(q[n], x);
-        own.template add<EV>(x, SelRow<T>::most_of(q[n], x));
+        own.template add<EV>(x, SelRow<T>::most_of(q[n], x), j + n * kSelThreads);
       }
   }
 }
@@ -218,99 +244,137 @@ struct SelSum {
 struct RowShared {
   uint64_t buffer[kSelBuffer], next[kSelWarps];
   double part_sum[kSelWarps];
-  float part_top[kSelWarps], bound[kSelWarps];
+  float part_top[kSelWarps];
+  uint32_t bound[kSelWarps];
   int column[kSelThreads];
   int found, columns;
 };
 
-template <typename T, int W>
-__device__ __forceinline__ void select_row(RowShared &sm, const SelRow<T> &row, int first, int end, bool edges,
-                                           SelSum *out, uint64_t *list, int beam) {
+// a hypothesis: 0 none, 1 finished, 2 its row is read
+__device__ __forceinline__ int kind_of(float score, const uint8_t *finished, size_t at) {
+  return !(fabsf(score) < INFINITY) ? 0 : finished != nullptr && finished[at] != 0 ? 1 : 2;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kSelThreads, kSelResident)
+select_rows_kernel(const T *__restrict__ logits, long long batch, long long row_stride,
+                   const float *__restrict__ scores, const uint8_t *__restrict__ finished, int V,
+                   SelSum *__restrict__ sums, uint64_t *__restrict__ entries, int beam) {
   constexpr int EV = SelRow<T>::EV;
+  __shared__ RowShared sm;
+  // the second launch may be set up meanwhile; it waits for this one's end before it reads
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int part = blockIdx.x, parts = gridDim.x, i = blockIdx.y, K = gridDim.y, b = blockIdx.z;
+  const size_t at = (size_t)b * K + i, unit = at * parts + part;
+  const bool read = kind_of(scores[at], finished, at) == 2;
+  const int main_end = max(1, SelRow<T>::vectors(V) - 2), share = (main_end - 1 + parts - 1) / parts;
+  const int first = min(main_end, 1 + part * share), end = min(main_end, first + share);
+  const bool edges = part == 0;
+  const SelRow<T> row(logits + b * batch + i * row_stride, V);
+  SelSum *const out = sums + unit;
+  uint64_t *const list = entries + unit * beam;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   // an edge element for the lanes of the last warp, which have least of the row to read
   const int symbol = edges && warp == kSelWarps - 1 ? row.edge_symbol(lane) : -1;
-  const float edge = symbol >= 0 ? in_f32(row.row[symbol]) : neg_inf<float>();
+  float edge = symbol >= 0 ? in_f32(row.row[symbol]) : neg_inf<float>();
   SelShare own;
-  stream_row<T, W>(own, row, first, end);
+  switch (row.words()) {
+    case -1: stream_row<T, -1>(own, row, first, end, read); break;
+    case 0: stream_row<T, 0>(own, row, first, end, read); break;
+    case 1: stream_row<T, 1>(own, row, first, end, read); break;
+    case 2: stream_row<T, 2>(own, row, first, end, read); break;
+    default: stream_row<T, 3>(own, row, first, end, read); break;
+  }
+  if (!read) return;
   const float column_top = own.top;
+  const int column_at = own.at;
+  const float column_next = own.next;
   if (symbol >= 0) {
     const float x[2] = {edge, neg_inf<float>()};
-    own.template add<2>(x, edge);
+    own.template add<2>(x, edge, 0);
   }
-  const float warp_top = warp_max(own.top);
-  const float warp_total = warp_sum(own.relative() * exp_below(own.top, warp_top));
   // bound
   const int whole = min(kSelWarps, max(1, (end - first) / 32));   // warps whose lanes all have a share
-  const float mth = mth_of_warp(own.top, (beam + whole - 1) / whole);
+  uint32_t left = ordered(own.top);
+  const uint32_t most = __reduce_max_sync(0xffffffffu, left);
+  uint32_t mth = most;
+  for (int n = 1; n < (beam + whole - 1) / whole; ++n) {
+    if (lane == __ffs(__ballot_sync(0xffffffffu, left == mth)) - 1) left = 0;
+    mth = __reduce_max_sync(0xffffffffu, left);
+  }
+  const float warp_top = unordered(most);
+  const float warp_total = warp_sum(own.relative() * exp_below(own.top, warp_top));
   if (lane == 0) {
     sm.part_top[warp] = warp_top;
     sm.part_sum[warp] = warp_total;
-    sm.bound[warp] = warp < whole ? mth : INFINITY;
+    sm.bound[warp] = warp < whole ? mth : 0xffffffffu;
   }
   if (tid == 0) sm.found = sm.columns = 0;
   if (tid < beam) list[tid] = 0;
   __syncthreads();
-  float bound = INFINITY;
+  uint32_t least = 0xffffffffu;
 #pragma unroll
-  for (int w = 0; w < kSelWarps; ++w) bound = fminf(bound, sm.bound[w]);
-  bound = fmaxf(bound, -FLT_MAX);   // -inf is no candidate
-  {
-    const bool chosen = column_top >= bound;
-    const unsigned all = __ballot_sync(0xffffffffu, chosen);
-    int slot = lane == 0 && all ? atomicAdd(&sm.columns, __popc(all)) : 0;
-    slot = __shfl_sync(0xffffffffu, slot, 0) + __popc(all & ((1u << lane) - 1));
-    if (chosen) sm.column[slot] = tid;
-  }
-  if (tid == 0) {
-    float m = neg_inf<float>();
-    double sum = 0;
-#pragma unroll
-    for (int w = 0; w < kSelWarps; ++w) m = fmaxf(m, sm.part_top[w]);
-#pragma unroll
-    for (int w = 0; w < kSelWarps; ++w) sum += sm.part_sum[w] * (double)exp_below(sm.part_top[w], m);
-    out->top = m;
-    out->sum = sum;
-  }
-  __syncthreads();
+  for (int w = 0; w < kSelWarps; ++w) least = min(least, sm.bound[w]);
+  const float bound = unordered(max(least, ordered(-FLT_MAX)));   // -inf is no candidate
   // collect
-  const int pairs = sm.columns * ((end - first + kSelThreads - 1) / kSelThreads);
-  const auto collect = [&](auto &&take) {
-    if (edge >= bound) take(entry_of(edge, (uint32_t)symbol));
-    const int columns = sm.columns;
-    for (int p = tid; p < pairs; p += kSelThreads) {
-      const int level = p / columns, j = first + sm.column[p - level * columns] + level * kSelThreads;
-      if (j >= end) continue;
-      const uint4 q = row.template load<W>(j);
-      float x[EV];
-      SelRow<T>::unpack(q, x);
-      if (!(SelRow<T>::most_of(q, x) >= bound)) continue;
-#pragma unroll
-      for (int e = 0; e < EV; ++e)
-        if (x[e] >= bound) take(entry_of(x[e], (uint32_t)(j * EV + e)));
-    }
-  };
-  collect([&](uint64_t e) {
+  const auto push = [&](uint64_t e) {
     const int n = atomicAdd(&sm.found, 1);
     if (n < kSelBuffer) sm.buffer[n] = e;
-  });
+  };
+  const auto look = [&](int j, auto &&take) {
+    const uint4 q = load_any(row, j);
+    float x[EV];
+    SelRow<T>::unpack(q, x);
+    unsigned reach = 0;
+#pragma unroll
+    for (int e = 0; e < EV; ++e) reach |= (unsigned)(x[e] >= bound) << e;
+    for (; reach != 0; reach &= reach - 1) {   // mostly one
+      const int at = __ffs(reach) - 1;
+      float v = x[0];
+#pragma unroll
+      for (int e = 1; e < EV; ++e) v = e == at ? x[e] : v;
+      take(entry_of(v, (uint32_t)(j * EV + at)));
+    }
+  };
+  if (column_top >= bound) {
+    if (column_next >= bound) sm.column[atomicAdd(&sm.columns, 1)] = tid;
+    else look(column_at, push);
+  }
+  if (edge >= bound) push(entry_of(edge, (uint32_t)symbol));
+  if (warp == kSelWarps - 2 && lane < kSelWarps) {   // the row's maximum and sum
+    const unsigned mask = (1u << kSelWarps) - 1;
+    const float mine = sm.part_top[lane], m = unordered(__reduce_max_sync(mask, ordered(mine)));
+    double sum = sm.part_sum[lane] * (double)exp_below(mine, m);
+#pragma unroll
+    for (int o = kSelWarps / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(mask, sum, o);
+    if (lane == 0) out->top = m, out->sum = sum;
+  }
   __syncthreads();
+  const int columns = sm.columns, pairs = columns * ((end - first + kSelThreads - 1) / kSelThreads);
+  for (int p = tid; p < pairs; p += kSelThreads) {
+    const int level = p / columns, j = first + sm.column[p - level * columns] + level * kSelThreads;
+    if (j < end) look(j, push);
+  }
+  if (columns > 0) __syncthreads();
   const int found = sm.found;
   if (found <= kSelBuffer) {
-    // order: a warp for each
-    for (int c = warp; c < found; c += kSelWarps) {
+    // order
+    for (int c = tid; c < found; c += kSelThreads) {
       const uint64_t mine = sm.buffer[c];
       int earlier = 0;
-      for (int o = lane; o < found; o += 32) earlier += sm.buffer[o] > mine;
-      earlier = __reduce_add_sync(0xffffffffu, earlier);
-      if (lane == 0 && earlier < beam) list[earlier] = mine;
+#pragma unroll 8
+      for (int o = 0; o < found; ++o) earlier += sm.buffer[o] > mine;
+      if (earlier < beam) list[earlier] = mine;
     }
   } else {
     // more than the buffer holds (equal logits, or the best ones in few columns): one at a time
     uint64_t last = ~0ull;
     for (int n = 0; n < beam; ++n) {
       uint64_t best = 0;
-      collect([&](uint64_t e) { best = e < last && e > best ? e : best; });
+      const auto keep = [&](uint64_t e) { best = e < last && e > best ? e : best; };
+      if (edge >= bound) keep(entry_of(edge, (uint32_t)symbol));
+      if (column_top >= bound)
+        for (int j = first + tid; j < end; j += kSelThreads) look(j, keep);
       for (int o = 16; o > 0; o >>= 1) {
         const uint64_t other = __shfl_xor_sync(0xffffffffu, best, o);
         best = other > best ? other : best;
@@ -322,34 +386,6 @@ __device__ __forceinline__ void select_row(RowShared &sm, const SelRow<T> &row, 
       last = best;
       __syncthreads();
     }
-  }
-}
-
-// a hypothesis: 0 none, 1 finished, 2 its row is read
-__device__ __forceinline__ int kind_of(float score, const uint8_t *finished, size_t at) {
-  return !(fabsf(score) < INFINITY) ? 0 : finished != nullptr && finished[at] != 0 ? 1 : 2;
-}
-
-template <typename T>
-__global__ void __launch_bounds__(kSelThreads, 4)
-select_rows_kernel(const T *__restrict__ logits, long long batch, long long row_stride,
-                   const float *__restrict__ scores, const uint8_t *__restrict__ finished, int V,
-                   SelSum *__restrict__ sums, uint64_t *__restrict__ entries, int beam) {
-  __shared__ RowShared sm;
-  const int part = blockIdx.x, parts = gridDim.x, i = blockIdx.y, K = gridDim.y, b = blockIdx.z;
-  const size_t at = (size_t)b * K + i, unit = at * parts + part;
-  if (kind_of(scores[at], finished, at) != 2) return;
-  const int main_end = max(1, SelRow<T>::vectors(V) - 2), share = (main_end - 1 + parts - 1) / parts;
-  const int first = min(main_end, 1 + part * share), end = min(main_end, first + share);
-  const SelRow<T> row(logits + b * batch + i * row_stride, V);
-  SelSum *const sum = sums + unit;
-  uint64_t *const list = entries + unit * beam;
-  switch (row.words()) {
-    case -1: select_row<T, -1>(sm, row, first, end, part == 0, sum, list, beam); break;
-    case 0: select_row<T, 0>(sm, row, first, end, part == 0, sum, list, beam); break;
-    case 1: select_row<T, 1>(sm, row, first, end, part == 0, sum, list, beam); break;
-    case 2: select_row<T, 2>(sm, row, first, end, part == 0, sum, list, beam); break;
-    default: select_row<T, 3>(sm, row, first, end, part == 0, sum, list, beam); break;
   }
 }
 
@@ -377,6 +413,11 @@ select_join_kernel(const SelSum *__restrict__ sums, const uint64_t *__restrict__
   const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const SelSum *const sum = sums + (size_t)b * K * parts;
   const uint64_t *const list = entries + (size_t)b * K * parts * beam;
+  // Neighbouring entries go to different warps: every warp then has about the same share of good
+  // ones, and the least of their m-th best is a close bound.
+  const int each_row = parts * beam, all = K * each_row, own = lane * kSelWarps + warp;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const uint64_t first_entry = own < all ? list[own] : 0;   // whether it is needed or not
   // a row's log-sum.  A finished row is one whose only entry has logit and log-sum 0.
   float widest = 0;
   for (int i = tid; i < K; i += kSelThreads) {
@@ -402,21 +443,20 @@ select_join_kernel(const SelSum *__restrict__ sums, const uint64_t *__restrict__
   }
   if (tid == 0) found = 0;
   __syncthreads();
-  const int each_row = parts * beam;
   const auto entry = [&](int n, int &i, bool &done) {   // the n-th of K x parts x beam; 0: none
     i = n / each_row;
     if (row_shift[i] == neg_inf<float>()) return (uint64_t)0;
     done = finished != nullptr && finished[(size_t)b * K + i] != 0;
-    return !done ? list[n] : n == i * each_row ? entry_of(0.0f, (uint32_t)blank) : (uint64_t)0;
+    return !done ? (n < kSelThreads ? first_entry : list[n]) : n == i * each_row ? entry_of(0.0f, (uint32_t)blank) : (uint64_t)0;
   };
   float best = neg_inf<float>();
-  for (int n = tid; n < K * each_row; n += kSelThreads) {
+  for (int n = own; n < all; n += kSelThreads) {
     int i;
     bool done;
     const uint64_t e = entry(n, i, done);
     if (e != 0) best = fmaxf(best, logit_of(e) + row_shift[i]);
   }
-  const int whole = min(kSelWarps, max(1, K * each_row / 32));
+  const int whole = min(kSelWarps, all);   // warps that have entries
   const float mth = mth_of_warp(best, (beam + whole - 1) / whole);
   widest = warp_max(widest);
   if (lane == 0) warp_bound[warp] = warp < whole ? mth : INFINITY, warp_widest[warp] = widest;
@@ -429,7 +469,7 @@ select_join_kernel(const SelSum *__restrict__ sums, const uint64_t *__restrict__
   bound -= 4.0f * 0x1p-23f * (fabsf(bound) + widest);
   if (!(widest < 1e30f)) bound = neg_inf<float>();
   const auto collect = [&](auto &&take) {
-    for (int n = tid; n < K * each_row; n += kSelThreads) {
+    for (int n = own; n < all; n += kSelThreads) {
       int i;
       bool done;
       const uint64_t e = entry(n, i, done);
@@ -456,12 +496,12 @@ select_join_kernel(const SelSum *__restrict__ sums, const uint64_t *__restrict__
     out_parents[o] = out_tokens[o] = -1;
   }
   if (found <= kSelBuffer) {
-    for (int c = warp; c < found; c += kSelWarps) {
+    for (int c = tid; c < found; c += kSelThreads) {
       const SelEntry mine = {key[c], place[c]};
       int earlier = 0;
-      for (int o = lane; o < found; o += 32) earlier += before({key[o], place[o]}, mine);
-      earlier = __reduce_add_sync(0xffffffffu, earlier);
-      if (lane == 0 && earlier < beam) write(earlier, mine);
+#pragma unroll 4
+      for (int o = 0; o < found; ++o) earlier += before({key[o], place[o]}, mine);
+      if (earlier < beam) write(earlier, mine);
     }
     return;
   }
@@ -536,10 +576,18 @@ static int select_launch(const T *logits, long long batch, long long row, const 
   FRNNT_KERNEL(select_rows_kernel<T><<<dim3((unsigned)parts, (unsigned)K, (unsigned)B), kSelThreads, 0, st>>>(
       logits, batch, row, scores, finished, V, sums, entries, beam));
   FRNNT_CUDA(cudaGetLastError());
-  FRNNT_KERNEL(select_join_kernel<<<(unsigned)B, kSelThreads, 0, st>>>(sums, entries, scores, finished, blank,
-                                                                       out_scores, out_parents, out_tokens, K, V,
-                                                                       parts, beam));
-  FRNNT_CUDA(cudaGetLastError());
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3((unsigned)B);
+  config.blockDim = dim3(kSelThreads);
+  config.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = attr;
+  config.numAttrs = 1;
+  FRNNT_CUDA(FRNNT_KERNEL(cudaLaunchKernelEx(&config, select_join_kernel, (const SelSum *)sums,
+                                             (const uint64_t *)entries, scores, finished, blank, out_scores,
+                                             out_parents, out_tokens, K, V, parts, beam)));
   return FRNNT_OK;
 }
 

@@ -19,6 +19,7 @@
 // itself, so that no barrier belongs to the copies.
 #include <cooperative_groups.h>
 
+#include <atomic>
 #include <climits>
 
 #include "common.cuh"
@@ -26,7 +27,7 @@
 
 namespace frnnt {
 
-constexpr int kRecMostCluster = 8;
+constexpr int kRecMostCluster = 16;   // more than the portable eight: long sequences of few channels
 
 // ---- copies to shared memory ---------------------------------------------------------
 template <int BYTES> __device__ __forceinline__ void copy_async(void *to, const void *from) {
@@ -44,15 +45,18 @@ template <int LEFT> __device__ __forceinline__ void copy_wait() {
 }
 
 // One input's tile: kSteps vectors per thread, at [step][thread], so that a warp's accesses are
-// contiguous.  Values of two bytes that no wider vector reaches are loaded and stored instead
-// (cp.async moves 4, 8 or 16 bytes).
+// contiguous; steps from n on are filled with `pad`.  Values of two bytes that no wider vector
+// reaches are loaded and stored instead (cp.async moves 4, 8 or 16 bytes).
 template <typename S> struct RecTile {
   using T = typename S::T;
   using Pack = RecPack<T, S::VEC>;
-  __device__ static void fetch(Pack *tile, const T *from, long long step, int first, int n) {
+  __device__ static void fetch(Pack *tile, const T *from, long long step, int first, int n, const Pack &pad) {
 #pragma unroll
     for (int s = 0; s < S::kSteps; ++s) {
-      if (first + s >= n) break;
+      if (first + s >= n) {
+        tile[s * kRecThreads] = pad;
+        continue;
+      }
       const T *p = from + (first + s) * step;
       if constexpr (sizeof(Pack) == 2)
         tile[s * kRecThreads] = *reinterpret_cast<const Pack *>(p);
@@ -74,9 +78,10 @@ template <typename S> struct RecPlace {
     c = lane % S::LC * S::VEC;
     channel = tile * S::kWidth + c;
     inside = channel < D;    // D is a multiple of VEC
-    joiner = tid < S::kJoiners;
-    join_q = S::kJoin == 1 ? 0 : lane >> 3;
-    join_c = S::kJoin == 1 ? tid : warp * 8 + (lane & 7);
+    // eight channels to a segment of lanes, their kJoin runs eight lanes apart
+    join_q = lane / 8 % S::kJoin;
+    join_c = (warp * (32 / S::kSegment) + lane / S::kSegment) * 8 + lane % 8;
+    joiner = join_c < S::kWidth;
   }
 };
 
@@ -112,38 +117,103 @@ template <typename real, int VEC> __device__ __forceinline__ void get(const real
   }
 }
 
-// The state that a tile starts from, and the one after all tiles of the cluster's turn: `carry`
-// is the state before the turn, (A, B) the composition of this CTA's tile, slots [ranks][2][width]
-// where every CTA leaves its own in every CTA.  FORWARD: in the order of the ranks, else against.
-template <typename S, bool FORWARD>
-__device__ __forceinline__ typename S::real
-join_cluster(typename S::real A, typename S::real B, typename S::real &carry, typename S::real *slots, int rank,
-             int ranks, const RecPlace<S> &at) {
-  using real = typename S::real;
-  namespace cg = cooperative_groups;
-  cg::cluster_group cluster = cg::this_cluster();
-  if (at.joiner) {
-    for (int r = at.join_q; r < ranks; r += S::kJoin) {
-      real *peer = cluster.map_shared_rank(slots, r) + rank * 2 * S::kWidth + at.join_c;
-      peer[0] = A;
-      peer[S::kWidth] = B;
-    }
+// ---- the tiles of a cluster --------------------------------------------------------------
+// Every CTA sends the composition of its tile to every CTA, straight into its shared memory and
+// counted there by an mbarrier (st.async: a cluster barrier would wait for the stores of h or of
+// the gradients too, a microsecond a turn).  Two buffers in turn are enough: who sends for turn
+// n + 2 has received everybody's composition of turn n + 1, which they sent after they had read
+// turn n's.  Waits are bounded; one that runs out makes the CTA go on with NaN for the state,
+// which reaches all that depends on it.
+constexpr int kRecTries = 1 << 20;
+
+struct RecMail {
+  void *slots;       // [2][ranks][kWidth][2]
+  uint64_t *bars;    // [2]
+  int rank, ranks;
+  bool failed;
+};
+__device__ __forceinline__ uint32_t peer_address(const void *p, int rank) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
+  return a;
+}
+__device__ __forceinline__ void send_pair(uint32_t to, float a, float b, uint32_t bar) {
+  asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v2.b32 [%0], {%1, %2}, [%3];" ::"r"(to),
+               "r"(__float_as_uint(a)), "r"(__float_as_uint(b)), "r"(bar)
+               : "memory");
+}
+__device__ __forceinline__ void send_pair(uint32_t to, double a, double b, uint32_t bar) {
+  asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v2.b64 [%0], {%1, %2}, [%3];" ::"r"(to),
+               "l"(__double_as_longlong(a)), "l"(__double_as_longlong(b)), "r"(bar)
+               : "memory");
+}
+__device__ __forceinline__ void mail_begin(const RecMail &mail) {
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i)
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"((uint32_t)__cvta_generic_to_shared(mail.bars + i)) : "memory");
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  cluster.sync();
+  cooperative_groups::this_cluster().sync();   // all have started, and have their mbarriers
+}
+// Nobody leaves before all have received what was sent to them.  A CTA that gave up waiting has not
+// seen its last values arrive: it stays some fifty times as long as they are under way at most.
+__device__ __forceinline__ void mail_end(const RecMail &mail) {
+  const bool failed = __syncthreads_or(mail.failed);
+  cooperative_groups::this_cluster().sync();
+  for (int i = 0; failed && i < 64; ++i) __nanosleep(1000);
+}
+// The composition (A, B) of this CTA's tile to all, in the n-th turn.  For joiners.
+template <typename S>
+__device__ __forceinline__ void mail_send(typename S::real A, typename S::real B, int n, const RecMail &mail,
+                                          const RecPlace<S> &at) {
+  using real = typename S::real;
+  const int buffer = n & 1;
+  const real *slots = (const real *)mail.slots + buffer * mail.ranks * 2 * S::kWidth;
+  if (threadIdx.x == 0)
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(
+                     (uint32_t)__cvta_generic_to_shared(mail.bars + buffer)),
+                 "r"(mail.ranks * 2 * S::kWidth * (int)sizeof(real))
+                 : "memory");
+  for (int r = at.join_q; r < mail.ranks; r += S::kJoin)
+    send_pair(peer_address(slots + (mail.rank * S::kWidth + at.join_c) * 2, r), A, B,
+              peer_address(mail.bars + buffer, r));
+}
+// The state that the tile starts from.  `carry`: the state before the n-th turn, and after it on
+// return.  FORWARD: in the order of the ranks, else against it.  For joiners.
+template <typename S, bool FORWARD>
+__device__ __forceinline__ typename S::real mail_join(typename S::real &carry, int n, RecMail &mail,
+                                                      const RecPlace<S> &at) {
+  using real = typename S::real;
+  const int buffer = n & 1;
+  const real *slots = (const real *)mail.slots + buffer * mail.ranks * 2 * S::kWidth;
+  const uint32_t bar = (uint32_t)__cvta_generic_to_shared(mail.bars + buffer);
+  bool arrived = false;
+  for (int i = 0; !mail.failed && !arrived && i < kRecTries; ++i) {
+    uint32_t done;
+    asm volatile("{\n.reg .pred q;\nmbarrier.try_wait.parity.shared::cta.b64 q, [%1], %2;\n"
+                 "selp.u32 %0, 1, 0, q;\n}"
+                 : "=r"(done)
+                 : "r"(bar), "r"((n >> 1) & 1)
+                 : "memory");
+    arrived = done != 0;
+  }
+  if (!arrived) {
+    mail.failed = true;
+    return carry = real(NAN);
+  }
   real before = carry;
-  if (at.joiner) {
-    for (int i = 0; i < ranks; ++i) {
-      const int r = FORWARD ? i : ranks - 1 - i;
-      if (r == rank) before = carry;
-      const real *own = slots + r * 2 * S::kWidth + at.join_c;
-      carry = own[0] * carry + own[S::kWidth];
-    }
+#pragma unroll 4
+  for (int i = 0; i < mail.ranks; ++i) {
+    const int r = FORWARD ? i : mail.ranks - 1 - i;
+    if (r == mail.rank) before = carry;
+    const real *own = slots + (r * S::kWidth + at.join_c) * 2;
+    carry = own[0] * carry + own[1];
   }
   return before;
 }
 
 template <typename S, bool CLUSTER>
-__global__ void __launch_bounds__(kRecThreads)
+__global__ void __launch_bounds__(kRecThreads, 4)
 recurrence_forward_kernel(RecTensor x, RecTensor gate, const typename S::real *__restrict__ initial,
                           const int64_t *__restrict__ lengths, typename S::T *__restrict__ h,
                           typename S::real *__restrict__ last, typename S::real *__restrict__ saved, int steps,
@@ -155,8 +225,9 @@ recurrence_forward_kernel(RecTensor x, RecTensor gate, const typename S::real *_
   extern __shared__ __align__(16) unsigned char smem[];
   Pack *const tiles = reinterpret_cast<Pack *>(smem) + threadIdx.x;        // [2][x, gate][STEPS][thread]
   real *const exchange = reinterpret_cast<real *>(smem + 4 * S::kStage);   // [2][A, B][kExchange]
-  real *const slots = exchange + 4 * S::kExchange;                         // [2][ranks][2][kWidth]
   const int rank = CLUSTER ? blockIdx.x : 0, ranks = CLUSTER ? gridDim.x : 1;
+  real *const slots = exchange + 4 * S::kExchange;
+  RecMail mail{slots, reinterpret_cast<uint64_t *>(slots + 4 * ranks * S::kWidth), rank, ranks, false};
   const int b = blockIdx.z;
   const RecPlace<S> at(blockIdx.y, D);
   const int n = steps_of(lengths, b, steps), chunks = (steps + kRecChunk - 1) / kRecChunk;
@@ -167,19 +238,19 @@ recurrence_forward_kernel(RecTensor x, RecTensor gate, const typename S::real *_
   const bool keeper = at.joiner && join_channel < D;
   real carry = keeper && initial != nullptr ? initial[(size_t)b * D + join_channel] : real(0);
   const int turns = (n + kRecChunk * ranks - 1) / (kRecChunk * ranks);
-  const int piece_first = at.piece * STEPS;
+  const int piece_first = at.piece * STEPS, here = at.inside ? n : 0;   // steps that this thread has
 
   const auto fetch = [&](int turn) {
     const int first = (turn * ranks + rank) * kRecChunk + piece_first;
     Pack *tile = tiles + (turn & 1) * 2 * STEPS * kRecThreads;
-    if (at.inside && turn < turns) {
-      RecTile<S>::fetch(tile, X, x.step, first, n);
-      RecTile<S>::fetch(tile + STEPS * kRecThreads, G, gate.step, first, n);
+    if (turn < turns) {   // behind the sequence, a gate that keeps the state as it is
+      RecTile<S>::fetch(tile, X, x.step, first, here, rec_fill<T, VEC>(0.0f));
+      RecTile<S>::fetch(tile + STEPS * kRecThreads, G, gate.step, first, here, rec_fill<T, VEC>(INFINITY));
     }
     copy_commit();
   };
   fetch(0);
-  if constexpr (CLUSTER) cooperative_groups::this_cluster().sync();   // all have started
+  if constexpr (CLUSTER) mail_begin(mail);
   for (int turn = 0; turn < turns; ++turn) {
     fetch(turn + 1);
     copy_wait<1>();
@@ -188,21 +259,19 @@ recurrence_forward_kernel(RecTensor x, RecTensor gate, const typename S::real *_
     real f[STEPS][VEC], u[STEPS][VEC], A[VEC], B[VEC];
     const Pack *tile = tiles + (turn & 1) * 2 * STEPS * kRecThreads;
 #pragma unroll
-    for (int k = 0; k < VEC; ++k) A[k] = real(1), B[k] = real(0);
-#pragma unroll
     for (int s = 0; s < STEPS; ++s) {
-      const bool live = at.inside && first + s < n;
-      real xv[VEC], gv[VEC];
+      real xv[VEC], gv[VEC], take[VEC];
       rec_unpack<T, VEC>(tile[s * kRecThreads], xv);
       rec_unpack<T, VEC>(tile[(STEPS + s) * kRecThreads], gv);
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) {
-        real keep, take;
-        gate_pair<T>(gv[k], keep, take);
-        f[s][k] = live ? keep : real(1);
-        u[s][k] = live ? take * xv[k] : real(0);
-        A[k] *= f[s][k];
-        B[k] = f[s][k] * B[k] + u[s][k];
+      for (int k = 0; k < VEC; ++k) gate_pair<T>(gv[k], f[s][k], take[k]);
+      vmul(u[s], take, xv);
+      if (s == 0) {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) A[k] = f[0][k], B[k] = u[0][k];
+      } else {
+        vmul(A, A, f[s]);
+        vfma(B, f[s], B, u[s]);
       }
     }
     put<real, VEC>(EA + S::at(at.piece, at.c), A);
@@ -224,23 +293,23 @@ recurrence_forward_kernel(RecTensor x, RecTensor gate, const typename S::real *_
     if constexpr (S::kJoin > 1) {
 #pragma unroll
       for (int o = 1; o < S::kJoin; o *= 2) {
-        const real pa = __shfl_up_sync(0xffffffffu, a, 8 * o), pb = __shfl_up_sync(0xffffffffu, bb, 8 * o);
+        const real pa = __shfl_up_sync(0xffffffffu, a, 8 * o, S::kSegment), pb = __shfl_up_sync(0xffffffffu, bb, 8 * o, S::kSegment);
         if (at.join_q >= o) {
           bb = a * pb + bb;
           a *= pa;
         }
       }
-      const real pa = __shfl_up_sync(0xffffffffu, a, 8), pb = __shfl_up_sync(0xffffffffu, bb, 8);
+      const real pa = __shfl_up_sync(0xffffffffu, a, 8, S::kSegment), pb = __shfl_up_sync(0xffffffffu, bb, 8, S::kSegment);
       if (at.join_q > 0) ex_a = pa, ex_b = pb;
-      a = __shfl_sync(0xffffffffu, a, 8 * (S::kJoin - 1) + (threadIdx.x & 7));
-      bb = __shfl_sync(0xffffffffu, bb, 8 * (S::kJoin - 1) + (threadIdx.x & 7));
+      a = __shfl_sync(0xffffffffu, a, S::kSegment - 8 + (threadIdx.x & 7), S::kSegment);
+      bb = __shfl_sync(0xffffffffu, bb, S::kSegment - 8 + (threadIdx.x & 7), S::kSegment);
     }
-    real start = carry;
     if constexpr (CLUSTER)
-      start = join_cluster<S, true>(a, bb, carry, slots + (turn & 1) * ranks * 2 * S::kWidth, rank, ranks, at);
-    else
-      carry = a * carry + bb;
+      if (at.joiner) mail_send(a, bb, turn, mail, at);
     if (at.joiner) {
+      real start = carry;
+      if constexpr (CLUSTER) start = mail_join<S, true>(carry, turn, mail, at);
+      else carry = a * carry + bb;
       if (saved != nullptr && at.join_q == 0 && keeper && chunk < chunks)
         saved[((size_t)b * chunks + chunk) * D + join_channel] = start;
       real state = ex_a * start + ex_b;
@@ -255,9 +324,8 @@ recurrence_forward_kernel(RecTensor x, RecTensor gate, const typename S::real *_
     get<real, VEC>(EB + S::at(at.piece, at.c), state);
 #pragma unroll
     for (int s = 0; s < STEPS; ++s) {
-#pragma unroll
-      for (int k = 0; k < VEC; ++k) state[k] = f[s][k] * state[k] + u[s][k];
-      if (at.inside && first + s < n)
+      vfma(state, f[s], state, u[s]);
+      if (first + s < here)
         *reinterpret_cast<Pack *>(H + (size_t)(first + s) * D) = rec_pack<T, VEC>(state);
     }
   }
@@ -267,10 +335,11 @@ recurrence_forward_kernel(RecTensor x, RecTensor gate, const typename S::real *_
       *reinterpret_cast<Pack *>(H + t * D) = rec_pack<T, VEC>(zero);
   }
   if (keeper && rank == 0 && at.join_q == 0) last[(size_t)b * D + join_channel] = carry;
+  if constexpr (CLUSTER) mail_end(mail);
 }
 
 template <typename S, bool CLUSTER>
-__global__ void __launch_bounds__(kRecThreads)
+__global__ void __launch_bounds__(kRecThreads, 3)
 recurrence_backward_kernel(RecTensor x, RecTensor gate, const int64_t *__restrict__ lengths,
                            const typename S::real *__restrict__ saved, RecTensor dh,
                            const typename S::real *__restrict__ dlast, typename S::T *__restrict__ dx,
@@ -283,66 +352,68 @@ recurrence_backward_kernel(RecTensor x, RecTensor gate, const int64_t *__restric
   extern __shared__ __align__(16) unsigned char smem[];
   Pack *const tiles = reinterpret_cast<Pack *>(smem) + threadIdx.x;        // [2][x, gate, dh][STEPS][thread]
   real *const exchange = reinterpret_cast<real *>(smem + 6 * S::kStage);   // [2][A, B, M][kExchange]
-  real *const slots = exchange + 6 * S::kExchange;                         // [2][ranks][2][kWidth]
   const int rank = CLUSTER ? blockIdx.x : 0, ranks = CLUSTER ? gridDim.x : 1;
+  real *const slots = exchange + 6 * S::kExchange;
+  RecMail mail{slots, reinterpret_cast<uint64_t *>(slots + 4 * ranks * S::kWidth), rank, ranks, false};
   const int b = blockIdx.z;
   const RecPlace<S> at(blockIdx.y, D);
   const int n = steps_of(lengths, b, steps), chunks = (steps + kRecChunk - 1) / kRecChunk;
   const T *const X = (const T *)x.data + b * x.batch + at.channel;
   const T *const G = (const T *)gate.data + b * gate.batch + at.channel;
-  const T *const DH = dh.data == nullptr ? nullptr : (const T *)dh.data + b * dh.batch + at.channel;
+  const T *const DH = (const T *)dh.data + b * dh.batch + at.channel;   // not read where there is none
   T *const DX = dx + (size_t)b * steps * D + at.channel, *const DG = dgate + (size_t)b * steps * D + at.channel;
   const int join_channel = blockIdx.y * S::kWidth + at.join_c;
   const bool keeper = at.joiner && join_channel < D;
   real carry = keeper && dlast != nullptr ? dlast[(size_t)b * D + join_channel] : real(0);
   const int turns = (n + kRecChunk * ranks - 1) / (kRecChunk * ranks);
-  const int piece_first = at.piece * STEPS;
+  const int piece_first = at.piece * STEPS, here = at.inside ? n : 0;   // steps that this thread has
 
   const auto fetch = [&](int turn) {
     const int first = (turn * ranks + rank) * kRecChunk + piece_first;
     Pack *tile = tiles + (turn & 1) * 3 * STEPS * kRecThreads;
-    if (at.inside && turn >= 0) {
-      RecTile<S>::fetch(tile, X, x.step, first, n);
-      RecTile<S>::fetch(tile + STEPS * kRecThreads, G, gate.step, first, n);
-      if (DH != nullptr) RecTile<S>::fetch(tile + 2 * STEPS * kRecThreads, DH, dh.step, first, n);
+    if (turn >= 0) {   // behind the sequence, a gate that keeps the state as it is
+      RecTile<S>::fetch(tile, X, x.step, first, here, rec_fill<T, VEC>(0.0f));
+      RecTile<S>::fetch(tile + STEPS * kRecThreads, G, gate.step, first, here, rec_fill<T, VEC>(INFINITY));
+      RecTile<S>::fetch(tile + 2 * STEPS * kRecThreads, DH, dh.step, first, dh.data == nullptr ? 0 : here,
+                        rec_fill<T, VEC>(0.0f));
     }
     copy_commit();
   };
   fetch(turns - 1);
-  if constexpr (CLUSTER) cooperative_groups::this_cluster().sync();   // all have started
+  if constexpr (CLUSTER) mail_begin(mail);
   for (int turn = turns - 1; turn >= 0; --turn) {
-    fetch(turn - 1);
+    if constexpr (!CLUSTER) fetch(turn - 1);
     const int chunk = turn * ranks + rank, first = chunk * kRecChunk + piece_first;
     real start = real(0);   // the state before the tile
     if (keeper && chunk * kRecChunk < n) start = saved[((size_t)b * chunks + chunk) * D + join_channel];
-    copy_wait<1>();
+    copy_wait<CLUSTER ? 0 : 1>();
     real *const EA = exchange + (turn & 1) * 3 * S::kExchange, *const EB = EA + S::kExchange,
                *const EM = EB + S::kExchange;
     real f[STEPS][VEC], take[STEPS][VEC], A[VEC], B[VEC], M[VEC];
     const Pack *tile = tiles + (turn & 1) * 3 * STEPS * kRecThreads;
 #pragma unroll
-    for (int k = 0; k < VEC; ++k) A[k] = real(1), B[k] = M[k] = real(0);
-#pragma unroll
     for (int s = 0; s < STEPS; ++s) {
-      const bool live = at.inside && first + s < n;
-      real xv[VEC], gv[VEC];
+      real xv[VEC], gv[VEC], u[VEC];
       rec_unpack<T, VEC>(tile[s * kRecThreads], xv);
       rec_unpack<T, VEC>(tile[(STEPS + s) * kRecThreads], gv);
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) {
-        gate_pair<T>(gv[k], f[s][k], take[s][k]);
-        f[s][k] = live ? f[s][k] : real(1);
-        A[k] *= f[s][k];
-        B[k] = f[s][k] * B[k] + (live ? take[s][k] * xv[k] : real(0));
+      for (int k = 0; k < VEC; ++k) gate_pair<T>(gv[k], f[s][k], take[s][k]);
+      vmul(u, take[s], xv);
+      if (s == 0) {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) A[k] = f[0][k], B[k] = u[k];
+      } else {
+        vmul(A, A, f[s]);
+        vfma(B, f[s], B, u);
       }
     }
+    vset(M, real(0));
 #pragma unroll
     for (int s = STEPS - 1; s >= 0; --s) {
-      const bool live = at.inside && first + s < n && DH != nullptr;
       real dv[VEC];
       rec_unpack<T, VEC>(tile[(2 * STEPS + s) * kRecThreads], dv);
-#pragma unroll
-      for (int k = 0; k < VEC; ++k) M[k] = f[s][k] * (M[k] + (live ? dv[k] : real(0)));
+      vadd(M, M, dv);
+      vmul(M, M, f[s]);
     }
     put<real, VEC>(EA + S::at(at.piece, at.c), A);
     put<real, VEC>(EB + S::at(at.piece, at.c), B);
@@ -368,8 +439,8 @@ recurrence_backward_kernel(RecTensor x, RecTensor gate, const int64_t *__restric
       real fa = a, sa = a;
 #pragma unroll
       for (int o = 1; o < S::kJoin; o *= 2) {
-        const real pa = __shfl_up_sync(0xffffffffu, fa, 8 * o), pb = __shfl_up_sync(0xffffffffu, bb, 8 * o);
-        const real na = __shfl_down_sync(0xffffffffu, sa, 8 * o), nm = __shfl_down_sync(0xffffffffu, m, 8 * o);
+        const real pa = __shfl_up_sync(0xffffffffu, fa, 8 * o, S::kSegment), pb = __shfl_up_sync(0xffffffffu, bb, 8 * o, S::kSegment);
+        const real na = __shfl_down_sync(0xffffffffu, sa, 8 * o, S::kSegment), nm = __shfl_down_sync(0xffffffffu, m, 8 * o, S::kSegment);
         if (at.join_q >= o) {
           bb = fa * pb + bb;
           fa *= pa;
@@ -379,19 +450,21 @@ recurrence_backward_kernel(RecTensor x, RecTensor gate, const int64_t *__restric
           sa *= na;
         }
       }
-      const real pa = __shfl_up_sync(0xffffffffu, fa, 8), pb = __shfl_up_sync(0xffffffffu, bb, 8);
-      const real na = __shfl_down_sync(0xffffffffu, sa, 8), nm = __shfl_down_sync(0xffffffffu, m, 8);
+      const real pa = __shfl_up_sync(0xffffffffu, fa, 8, S::kSegment), pb = __shfl_up_sync(0xffffffffu, bb, 8, S::kSegment);
+      const real na = __shfl_down_sync(0xffffffffu, sa, 8, S::kSegment), nm = __shfl_down_sync(0xffffffffu, m, 8, S::kSegment);
       if (at.join_q > 0) ex_a = pa, ex_b = pb;
       if (at.join_q + 1 < S::kJoin) af_a = na, af_m = nm;
-      a = __shfl_sync(0xffffffffu, sa, threadIdx.x & 7);   // of the whole tile
-      m = __shfl_sync(0xffffffffu, m, threadIdx.x & 7);
+      a = __shfl_sync(0xffffffffu, sa, threadIdx.x & 7, S::kSegment);   // of the whole tile
+      m = __shfl_sync(0xffffffffu, m, threadIdx.x & 7, S::kSegment);
     }
-    real flow = carry;
-    if constexpr (CLUSTER)
-      flow = join_cluster<S, false>(a, m, carry, slots + (turn & 1) * ranks * 2 * S::kWidth, rank, ranks, at);
-    else
-      carry = a * carry + m;
+    if constexpr (CLUSTER) {
+      if (at.joiner) mail_send(a, m, turns - 1 - turn, mail, at);
+      fetch(turn - 1);   // while the compositions are under way
+    }
     if (at.joiner) {
+      real flow = carry;
+      if constexpr (CLUSTER) flow = mail_join<S, false>(carry, turns - 1 - turn, mail, at);
+      else carry = a * carry + m;
       real state = ex_a * start + ex_b;
       flow = af_a * flow + af_m;
 #pragma unroll
@@ -411,27 +484,22 @@ recurrence_backward_kernel(RecTensor x, RecTensor gate, const int64_t *__restric
     get<real, VEC>(EM + S::at(at.piece, at.c), back);
 #pragma unroll
     for (int s = 0; s < STEPS; ++s) {
-      real xv[VEC];
+      real xv[VEC], u[VEC];
       rec_unpack<T, VEC>(tile[s * kRecThreads], xv);
-#pragma unroll
-      for (int k = 0; k < VEC; ++k) {
-        before[s][k] = state[k];
-        state[k] = f[s][k] * state[k] + take[s][k] * xv[k];
-      }
+      vsub(before[s], state, xv);   // h_{t-1} - x_t
+      vmul(u, take[s], xv);
+      vfma(state, f[s], state, u);
     }
 #pragma unroll
     for (int s = STEPS - 1; s >= 0; --s) {
-      if (!at.inside || first + s >= n) continue;
-      real xv[VEC], dv[VEC], ox[VEC], og[VEC];
-      rec_unpack<T, VEC>(tile[s * kRecThreads], xv);
+      if (first + s >= here) continue;
+      real dv[VEC], lam[VEC], ox[VEC], og[VEC];
       rec_unpack<T, VEC>(tile[(2 * STEPS + s) * kRecThreads], dv);
-#pragma unroll
-      for (int k = 0; k < VEC; ++k) {
-        const real lam = back[k] + (DH != nullptr ? dv[k] : real(0));
-        ox[k] = take[s][k] * lam;
-        og[k] = lam * (before[s][k] - xv[k]) * (f[s][k] * take[s][k]);
-        back[k] = f[s][k] * lam;
-      }
+      vadd(lam, back, dv);
+      vmul(back, f[s], lam);
+      vmul(ox, take[s], lam);
+      vmul(og, before[s], take[s]);
+      vmul(og, og, back);           // lam (h - x) f take
       *reinterpret_cast<Pack *>(DX + (size_t)(first + s) * D) = rec_pack<T, VEC>(ox);
       *reinterpret_cast<Pack *>(DG + (size_t)(first + s) * D) = rec_pack<T, VEC>(og);
     }
@@ -444,6 +512,7 @@ recurrence_backward_kernel(RecTensor x, RecTensor gate, const int64_t *__restric
     }
   }
   if (dinitial != nullptr && keeper && rank == 0 && at.join_q == 0) dinitial[(size_t)b * D + join_channel] = carry;
+  if constexpr (CLUSTER) mail_end(mail);
 }
 
 constexpr int kStepThreads = 128;
@@ -479,7 +548,7 @@ recurrence_step_kernel(const T *__restrict__ x, long long x_row, const T *__rest
 // multiprocessor a CTA, no more than the sequence has.
 static int ranks_for(long long ctas, int T) {
   int ranks = 1;
-  while (ranks < kRecMostCluster && ctas * ranks < sm_count() && 2 * ranks <= (T + kRecChunk - 1) / kRecChunk)
+  while (ranks < kRecMostCluster && ctas * ranks < 3 * sm_count() && 2 * ranks <= (T + kRecChunk - 1) / kRecChunk)
     ranks *= 2;
   return ranks;
 }
@@ -492,9 +561,19 @@ static int rec_launch(void (*alone)(Params...), void (*cluster)(Params...), int 
   FRNNT_REQUIRE(T <= INT_MAX - kRecMostCluster * kRecChunk, FRNNT_EUNSUPPORTED, "T too large");
   const int ranks = ranks_for((long long)B * tiles, T);
   const size_t smem = 2 * (size_t)arrays * (S::kStage + S::kExchange * sizeof(typename S::real)) +
-                      (ranks > 1 ? 4 * ranks * S::kWidth * sizeof(typename S::real) : 0);
+                      (ranks > 1 ? 4 * ranks * S::kWidth * sizeof(typename S::real) + 16 : 0);
   void (*kernel)(Params...) = ranks > 1 ? cluster : alone;
-  FRNNT_CUDA(cudaFuncSetAttribute((const void *)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  // the attribute belongs to the kernel on a device: asked for once, for the largest cluster
+  static std::atomic<uint64_t> allowed[2];
+  int dev = 0;
+  FRNNT_CUDA(cudaGetDevice(&dev));
+  const uint64_t bit = 1ull << (dev & 63);
+  if (dev > 63 || !(allowed[ranks > 1].load(std::memory_order_relaxed) & bit)) {
+    const size_t most = smem + (ranks > 1 ? 4 * (kRecMostCluster - ranks) * S::kWidth * sizeof(typename S::real) : 0);
+    FRNNT_CUDA(cudaFuncSetAttribute((const void *)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most));
+    if (ranks > 1) FRNNT_CUDA(cudaFuncSetAttribute((const void *)kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    allowed[ranks > 1].fetch_or(bit, std::memory_order_relaxed);
+  }
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3((unsigned)ranks, (unsigned)tiles, (unsigned)B);
   config.blockDim = dim3(kRecThreads);
@@ -533,21 +612,21 @@ static int backward_as(const RecTensor &x, const RecTensor &gate, const int64_t 
                        (typename S::T *)dgate, (real *)dinitial, T, D);
 }
 
-// Vectors of 16 bytes where every row allows them, eight lanes to the 128 bytes of a line; else
-// of 4 bytes (a float, or a pair of 16-bit values) where they do, else single values, 32 lanes
-// side by side.
+// Vectors of 16 bytes where every row allows them, else of 4 bytes (a float, or a pair of 16-bit
+// values) where they do, else single values; 64 or 128 bytes of a row side by side, and 32 values
+// a thread (16 doubles).
 #define FRNNT_REC_SHAPES(CALL, wide, pairs)                                              \
   switch (dtype) {                                                                       \
     case FRNNT_F32:                                                                      \
-      return wide ? CALL(RecShape<float, 4, 8>) : CALL(RecShape<float, 1, 32>);          \
+      return wide ? CALL(RecShape<float, 4, 8>) : CALL(RecShape<float, 1, 16>);          \
     case FRNNT_F64:                                                                      \
-      return wide ? CALL(RecShape<double, 2, 8>) : CALL(RecShape<double, 1, 32>);        \
+      return wide ? CALL(RecShape<double, 2, 8>) : CALL(RecShape<double, 1, 16>);        \
     case FRNNT_F16:                                                                      \
-      return wide ? CALL(RecShape<__half, 8, 8>)                                         \
-                  : pairs ? CALL(RecShape<__half, 2, 32>) : CALL(RecShape<__half, 1, 32>); \
+      return wide ? CALL(RecShape<__half, 8, 4>)                                         \
+                  : pairs ? CALL(RecShape<__half, 2, 16>) : CALL(RecShape<__half, 1, 32>); \
     default:                                                                             \
-      return wide ? CALL(RecShape<__nv_bfloat16, 8, 8>)                                  \
-                  : pairs ? CALL(RecShape<__nv_bfloat16, 2, 32>) : CALL(RecShape<__nv_bfloat16, 1, 32>); \
+      return wide ? CALL(RecShape<__nv_bfloat16, 8, 4>)                                  \
+                  : pairs ? CALL(RecShape<__nv_bfloat16, 2, 16>) : CALL(RecShape<__nv_bfloat16, 1, 32>); \
   }
 
 }  // namespace frnnt

@@ -1,5 +1,7 @@
 // Pieces of the gated linear recurrence: types, strided inputs, the gate, the shape of a tile.
 #pragma once
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace frnnt {
@@ -8,7 +10,7 @@ namespace frnnt {
 // per channel every 128 steps is 1.6 % of 16-bit values and gates, and the backward recomputes
 // a tile from its state instead of reading h.
 constexpr int kRecChunk = 128;
-constexpr int kRecThreads = 256;
+constexpr int kRecThreads = 128;
 constexpr int kRecWarps = kRecThreads / 32;
 
 // states, and everything computed, are 32 bits wide (64 for doubles)
@@ -53,30 +55,93 @@ __device__ __forceinline__ void rec_unpack(const RecPack<T, VEC> &p, RecState<T>
 #pragma unroll
   for (int k = 0; k < VEC; ++k) v[k] = rec_value<T>(e[k]);
 }
-template <typename T, int VEC> __device__ __forceinline__ RecPack<T, VEC> rec_pack(const RecState<T> (&v)[VEC]) {
+// a vector of one value
+template <typename T, int VEC> __device__ __forceinline__ RecPack<T, VEC> rec_fill(float value) {
   T e[VEC];
 #pragma unroll
-  for (int k = 0; k < VEC; ++k) e[k] = rec_round<T>(v[k]);
+  for (int k = 0; k < VEC; ++k) e[k] = T(value);
+  RecPack<T, VEC> p;
+  memcpy(&p, e, sizeof(p));
+  return p;
+}
+template <typename T, int VEC> __device__ __forceinline__ RecPack<T, VEC> rec_pack(const RecState<T> (&v)[VEC]) {
+  T e[VEC];
+  if constexpr (sizeof(T) == 2 && VEC % 2 == 0) {   // two at a time
+#pragma unroll
+    for (int k = 0; k < VEC; k += 2) {
+      if constexpr (std::is_same<T, __half>::value) {
+        const __half2 q = __floats2half2_rn(v[k], v[k + 1]);
+        e[k] = q.x, e[k + 1] = q.y;
+      } else {
+        const __nv_bfloat162 q = __floats2bfloat162_rn(v[k], v[k + 1]);
+        e[k] = q.x, e[k + 1] = q.y;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) e[k] = rec_round<T>(v[k]);
+  }
   RecPack<T, VEC> p;
   memcpy(&p, e, sizeof(p));
   return p;
 }
 
-// keep = sigmoid(g) and take = 1 - keep from one exponential of -|g|, which cannot overflow;
-// take is never the difference of two numbers near one.  16-bit inputs take the hardware's
-// exponential and division (relative error 2^-20, far below the 2^-9 / 2^-12 of their outputs).
-template <typename T> __device__ __forceinline__ void gate_pair(RecState<T> g, RecState<T> &keep, RecState<T> &take) {
-  using real = RecState<T>;
-  real e, r;
-  if constexpr (sizeof(T) == 2) {
-    e = __expf(-fabsf(g));
-    r = __fdividef(1.0f, 1.0f + e);
-  } else {
-    e = exp_r(-fabs(g));
-    r = real(1) / (real(1) + e);
+// ---- arithmetic on the channels of a thread: floats two at a time (half the instructions) -------
+#define FRNNT_REC_EACH(PAIR, ONE)                                              \
+  if constexpr (sizeof(real) == 4 && VEC % 2 == 0) {                           \
+    _Pragma("unroll") for (int k = 0; k < VEC; k += 2) {                       \
+      const float2 r = PAIR;                                                   \
+      out[k] = r.x, out[k + 1] = r.y;                                          \
+    }                                                                          \
+  } else {                                                                     \
+    _Pragma("unroll") for (int k = 0; k < VEC; ++k) out[k] = ONE;              \
   }
-  keep = g >= 0 ? r : e * r;
-  take = g >= 0 ? e * r : r;
+#define FRNNT_REC_PAIR(v) make_float2((float)v[k], (float)v[k + 1])
+template <typename real, int VEC>
+__device__ __forceinline__ void vmul(real (&out)[VEC], const real (&a)[VEC], const real (&b)[VEC]) {
+  FRNNT_REC_EACH(__fmul2_rn(FRNNT_REC_PAIR(a), FRNNT_REC_PAIR(b)), a[k] * b[k])
+}
+template <typename real, int VEC>
+__device__ __forceinline__ void vadd(real (&out)[VEC], const real (&a)[VEC], const real (&b)[VEC]) {
+  FRNNT_REC_EACH(__fadd2_rn(FRNNT_REC_PAIR(a), FRNNT_REC_PAIR(b)), a[k] + b[k])
+}
+template <typename real, int VEC>
+__device__ __forceinline__ void vfma(real (&out)[VEC], const real (&a)[VEC], const real (&b)[VEC], const real (&c)[VEC]) {
+  FRNNT_REC_EACH(__ffma2_rn(FRNNT_REC_PAIR(a), FRNNT_REC_PAIR(b), FRNNT_REC_PAIR(c)), a[k] * b[k] + c[k])
+}
+template <typename real, int VEC>   // a - b
+__device__ __forceinline__ void vsub(real (&out)[VEC], const real (&a)[VEC], const real (&b)[VEC]) {
+  FRNNT_REC_EACH(__ffma2_rn(FRNNT_REC_PAIR(b), make_float2(-1.0f, -1.0f), FRNNT_REC_PAIR(a)), a[k] - b[k])
+}
+template <typename real, int VEC> __device__ __forceinline__ void vset(real (&out)[VEC], real value) {
+#pragma unroll
+  for (int k = 0; k < VEC; ++k) out[k] = value;
+}
+#undef FRNNT_REC_EACH
+#undef FRNNT_REC_PAIR
+
+// keep = sigmoid(g) and take = 1 - keep from one exponential of -|g|, which cannot overflow;
+// take is never the difference of two numbers near one.  The reciprocal of 1 .. 2 is the
+// hardware's (within one unit in the last place); for 16-bit inputs the exponential is, too
+// (relative error 2^-20, far below the 2^-9 / 2^-12 of their outputs).
+template <typename T> __device__ __forceinline__ RecState<T> rec_exp(RecState<T> x) { return exp_r(x); }
+__device__ __forceinline__ float rec_exp_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x * 1.4426950408889634f));
+  return y;
+}
+template <> __device__ __forceinline__ float rec_exp<__half>(float x) { return rec_exp_fast(x); }
+template <> __device__ __forceinline__ float rec_exp<__nv_bfloat16>(float x) { return rec_exp_fast(x); }
+__device__ __forceinline__ float rec_reciprocal(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ double rec_reciprocal(double x) { return 1.0 / x; }
+template <typename T> __device__ __forceinline__ void gate_pair(RecState<T> g, RecState<T> &keep, RecState<T> &take) {
+  const RecState<T> e = rec_exp<T>(-fabs(g)), r = rec_reciprocal(1 + e), s = e * r;
+  keep = g >= 0 ? r : s;
+  take = g >= 0 ? s : r;
 }
 
 // ---- the tile of a CTA ------------------------------------------------------------
@@ -94,8 +159,8 @@ template <typename T_, int VEC_, int LC_> struct RecShape {
   // joining the pieces: kJoin threads per channel with kRun consecutive pieces each
   static constexpr int kRun = kPieces < 8 ? kPieces : 8;
   static constexpr int kJoin = kPieces / kRun;
-  static constexpr int kJoiners = kJoin * kWidth;
-  static_assert(kSteps * kPieces == kRecChunk && kJoiners <= kRecThreads && kJoin <= 4, "shape");
+  static constexpr int kSegment = 8 * kJoin;                    // lanes with all runs of eight channels
+  static_assert(kSteps * kPieces == kRecChunk && kJoin * kWidth <= kRecThreads && kJoin <= 4 && kWidth % 8 == 0, "shape");
   // offset of (piece, channel) in the exchange: runs are skewed by 8 so that the kJoin threads
   // of eight channels, which share a warp, hit different banks
   static __device__ __forceinline__ int at(int piece, int c) { return piece * kWidth + (piece / kRun) * 8 + c; }

@@ -9,7 +9,6 @@ from torch import Tensor
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._lib import _c_int, _c_longlong
 
 _CODES = {torch.float32: _lib.F32, torch.float64: _lib.F64, torch.float16: _lib.F16,
           torch.bfloat16: _lib.BF16}
@@ -31,57 +30,61 @@ def _rows(t: Tensor) -> Tensor:
     return t if t.shape[-1] <= 1 or t.stride(-1) == 1 else t.contiguous()
 
 
-def _strided(t: Optional[Tensor]):
-    """(pointer, batch stride, step stride) of a [B][T][D] tensor whose channels lie side by side"""
-    if t is None:
-        return None, _c_longlong(0), _c_longlong(0)
-    return _lib._c_vp(t.data_ptr()), _c_longlong(t.stride(0)), _c_longlong(t.stride(1))
-
-
 def _forward(x, gate, initial, lengths, keep_states):
     B, T, D = x.shape
-    dev, code = x.device, _code(x.dtype)
-    state = _state_type(x.dtype)
+    dev, code = x.device, _CODES[x.dtype]
     saved = None
     with _lib.on_device(dev):
-        h = torch.empty(B, T, D, dtype=x.dtype, device=dev)
-        last = torch.empty(B, D, dtype=state, device=dev)
+        h = torch.empty_like(x, memory_format=torch.contiguous_format)
+        last = x.new_empty((B, D), dtype=_state_type(x.dtype))
         if keep_states:
-            saved = torch.empty(max(_lib.size_of("frnnt_recurrence_saved_bytes", code, B, T, D), 1),
-                                dtype=torch.uint8, device=dev)
-        _lib.call("frnnt_recurrence_forward", _c_int(code), *_strided(x), *_strided(gate),
-                  _lib.ptr(initial), _lib.ptr(lengths), _lib.ptr(h), _lib.ptr(last),
-                  _lib.ptr(saved), B, T, D, _lib.stream_ptr(dev))
+            n = _lib.size_of("frnnt_recurrence_saved_bytes", code, B, T, D)
+            saved = x.new_empty(n, dtype=torch.uint8)
+        xs, gs = x.stride(), gate.stride()
+        _lib.call("frnnt_recurrence_forward", code, x.data_ptr(), xs[0], xs[1], gate.data_ptr(), gs[0],
+                  gs[1], None if initial is None else initial.data_ptr(),
+                  None if lengths is None else lengths.data_ptr(), h.data_ptr(), last.data_ptr(),
+                  None if saved is None else saved.data_ptr(), B, T, D, _lib.stream_ptr(dev))
     return h, last, saved
+
+
+def _backward(ctx, dh, dlast):
+    x, gate, lengths, saved = ctx.saved_tensors
+    B, T, D = x.shape
+    dev, code = x.device, _CODES[x.dtype]
+    if dh is not None:
+        dh = _rows(dh)
+    if dlast is not None:
+        dlast = dlast.contiguous()
+    with _lib.on_device(dev):
+        dx = torch.empty_like(x, memory_format=torch.contiguous_format)
+        dgate = torch.empty_like(dx)
+        dinitial = (x.new_empty((B, D), dtype=_state_type(x.dtype))
+                    if ctx.needs_input_grad[2] else None)
+        xs, gs, ds = x.stride(), gate.stride(), (0, 0) if dh is None else dh.stride()
+        _lib.call("frnnt_recurrence_backward", code, x.data_ptr(), xs[0], xs[1], gate.data_ptr(), gs[0],
+                  gs[1], None if lengths is None else lengths.data_ptr(), saved.data_ptr(),
+                  None if dh is None else dh.data_ptr(), ds[0], ds[1],
+                  None if dlast is None else dlast.data_ptr(), dx.data_ptr(), dgate.data_ptr(),
+                  None if dinitial is None else dinitial.data_ptr(), B, T, D, _lib.stream_ptr(dev))
+    return dx, dgate, dinitial, None
+
+
+_backward_once = once_differentiable(_backward)
 
 
 class _GatedRecurrence(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, gate, initial, lengths):
-        x, gate = _rows(x), _rows(gate)
         h, last, saved = _forward(x, gate, initial, lengths, True)
         ctx.save_for_backward(x, gate, lengths, saved)
         ctx.set_materialize_grads(False)
         return h, last
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dh, dlast):
-        x, gate, lengths, saved = ctx.saved_tensors
-        B, T, D = x.shape
-        dev, code = x.device, _code(x.dtype)
-        dh = None if dh is None else _rows(dh)
-        dlast = None if dlast is None else dlast.contiguous()
-        with _lib.on_device(dev):
-            dx = torch.empty(B, T, D, dtype=x.dtype, device=dev)
-            dgate = torch.empty(B, T, D, dtype=x.dtype, device=dev)
-            dinitial = (torch.empty(B, D, dtype=_state_type(x.dtype), device=dev)
-                        if ctx.needs_input_grad[2] else None)
-            _lib.call("frnnt_recurrence_backward", _c_int(code), *_strided(x), *_strided(gate),
-                      _lib.ptr(lengths), _lib.ptr(saved), *_strided(dh), _lib.ptr(dlast),
-                      _lib.ptr(dx), _lib.ptr(dgate), _lib.ptr(dinitial), B, T, D,
-                      _lib.stream_ptr(dev))
-        return dx, dgate, dinitial, None
+        # the wrapper that refuses a second derivative costs microseconds: only where one is recorded
+        return (_backward_once if torch.is_grad_enabled() else _backward)(ctx, dh, dlast)
 
 
 def gated_recurrence(x: Tensor, gate: Tensor, initial: Optional[Tensor] = None,
@@ -103,25 +106,26 @@ def gated_recurrence(x: Tensor, gate: Tensor, initial: Optional[Tensor] = None,
 
     Differentiable once with respect to x, gate and initial.  No counterpart in the reference."""
     assert x.ndim == 3, x.ndim
-    assert gate.shape == x.shape, (gate.shape, x.shape)
-    assert gate.dtype == x.dtype, (gate.dtype, x.dtype)
-    _code(x.dtype)
-    (B, T, D) = x.shape
-    state = _state_type(x.dtype)
-    assert x.is_cuda and gate.device == x.device, (x.device, gate.device)
+    shape, dtype, dev = x.shape, x.dtype, x.device
+    assert gate.shape == shape, (gate.shape, shape)
+    assert gate.dtype == dtype, (gate.dtype, dtype)
+    _code(dtype)
+    assert x.is_cuda and gate.device == dev, (dev, gate.device)
     if initial is not None:
-        assert initial.shape == (B, D), (initial.shape, (B, D))
-        assert initial.device == x.device, (initial.device, x.device)
-        assert initial.dtype in (state, x.dtype), initial.dtype
+        state = _state_type(dtype)
+        assert initial.shape == (shape[0], shape[2]), (initial.shape, shape)
+        assert initial.device == dev, (initial.device, dev)
+        assert initial.dtype in (state, dtype), initial.dtype
         initial = initial.to(state).contiguous()
     if lengths is not None:
-        assert lengths.shape == (B,) and lengths.dtype == torch.int64, (lengths.shape, lengths.dtype)
-        assert lengths.device == x.device, (lengths.device, x.device)
+        assert lengths.shape == shape[:1] and lengths.dtype == torch.int64, (lengths.shape, lengths.dtype)
+        assert lengths.device == dev, (lengths.device, dev)
         lengths = lengths.contiguous()
+    x, gate = _rows(x), _rows(gate)
     if torch.is_grad_enabled() and (x.requires_grad or gate.requires_grad or
                                     (initial is not None and initial.requires_grad)):
         return _GatedRecurrence.apply(x, gate, initial, lengths)
-    return _forward(_rows(x), _rows(gate), initial, lengths, False)[:2]
+    return _forward(x, gate, initial, lengths, False)[:2]
 
 
 def gated_recurrence_step(x: Tensor, gate: Tensor, state: Tensor,
@@ -157,16 +161,18 @@ def gated_recurrence_step(x: Tensor, gate: Tensor, state: Tensor,
     assert not (torch.is_grad_enabled() and (x.requires_grad or gate.requires_grad or
                                              state.requires_grad)), \
         "gated_recurrence_step has no gradients: use gated_recurrence, or torch.no_grad()"
-    x2, gate2 = _rows(x.reshape(-1, D)), _rows(gate.reshape(-1, D))
+    # rows at one distance from the next
+    x2 = x if x.is_contiguous() else _rows(x.reshape(-1, D))
+    gate2 = gate if gate.is_contiguous() else _rows(gate.reshape(-1, D))
     state = state.contiguous()
-    rows = x2.shape[0]
+    rows = x.numel() // D if D > 0 else 0
     with _lib.on_device(dev):
-        new = torch.empty(x.shape, dtype=kind, device=dev)
-        h = new if kind == x.dtype else torch.empty(x.shape, dtype=x.dtype, device=dev)
-        if rows > 0 and D > 0:
-            _lib.call("frnnt_recurrence_step", _c_int(code), _lib._c_vp(x2.data_ptr()),
-                      _c_longlong(x2.stride(0)), _lib._c_vp(gate2.data_ptr()),
-                      _c_longlong(gate2.stride(0)), _lib.ptr(state), _lib.ptr(parents),
-                      None if h is new else _lib.ptr(h), _lib.ptr(new), _c_longlong(rows), beams, K, D,
+        new = torch.empty_like(x, dtype=kind, memory_format=torch.contiguous_format)
+        h = new if kind == x.dtype else torch.empty_like(x, memory_format=torch.contiguous_format)
+        if rows > 0:
+            _lib.call("frnnt_recurrence_step", code, x2.data_ptr(), D if x2 is x else x2.stride(0),
+                      gate2.data_ptr(), D if gate2 is gate else gate2.stride(0), state.data_ptr(),
+                      None if parents is None else parents.data_ptr(),
+                      None if h is new else h.data_ptr(), new.data_ptr(), rows, beams, K, D,
                       _lib.stream_ptr(dev))
     return h, new
