@@ -81,31 +81,38 @@ def beam_reorder(states: Union[Tensor, Sequence[Tensor]], parents: Tensor) -> Un
     parents = parents.contiguous()
     if not tensors:
         return []
-    K, grad = None, torch.is_grad_enabled()
-    start, pitch, step, row = [], [], [], []
+    assert tensors[0].ndim >= 2 and tensors[0].shape[1] >= 1, tensors[0].shape
+    K, grad = tensors[0].shape[1], torch.is_grad_enabled()
+    start, target, pitch, step, row, out = [], [], [], [], [], []
+    held = []   # copies stay until the launch
+    shape = dtype = None
     with _lib.on_device(dev):
-        out = []
-        for n, t in enumerate(tensors):
-            shape = t.shape
-            assert len(shape) >= 2 and shape[0] == B, (shape, parents.shape)
-            K = shape[1] if n == 0 else K
-            assert shape[1] == K and K >= 1, (shape, K)
+        for t in tensors:
+            if t.shape != shape or t.dtype != dtype:   # tensors of one kind come in rows
+                shape, dtype = t.shape, t.dtype
+                assert len(shape) >= 2 and shape[0] == B and shape[1] == K, (shape, parents.shape, K)
+                size = t.element_size()
+                bytes_ = size * math.prod(shape[2:])
             assert t.device == dev, (t.device, dev)
             assert not (grad and t.requires_grad), \
                 "beam_reorder has no gradients: call it under torch.no_grad()"
-            # a row of a state has to lie in one piece; rows themselves may lie anywhere
-            if not t.is_contiguous() and B > 0 and not t[0, 0].is_contiguous():
-                t = tensors[n] = t.contiguous()
-            size, stride = t.element_size(), t.stride()
-            out.append(torch.empty_like(t, memory_format=torch.contiguous_format) if k == K
-                       else t.new_empty((B, k) + shape[2:]))
+            if t.is_contiguous():
+                pitch.append(K * bytes_)
+                step.append(bytes_)
+            else:   # a row of a state has to lie in one piece; rows themselves may lie anywhere
+                if B > 0 and not t[0, 0].is_contiguous():
+                    t = t.contiguous()
+                pitch.append(size * t.stride(0))
+                step.append(size * t.stride(1))
+                held.append(t)
+            new = (torch.empty_like(t, memory_format=torch.contiguous_format) if k == K
+                   else t.new_empty((B, k) + shape[2:]))
+            out.append(new)
             start.append(t.data_ptr())
-            pitch.append(size * stride[0])
-            step.append(size * stride[1])
-            row.append(size * math.prod(shape[2:]))
-        n = len(tensors)
+            target.append(new.data_ptr())
+            row.append(bytes_)
+        n = len(out)
         words, pointers = _c_longlong * n, _c_vp * n
         _lib.call("frnnt_beam_reorder", n, pointers(*start), words(*pitch), words(*step),
-                  pointers(*[t.data_ptr() for t in out]), words(*row), parents.data_ptr(), B, k, K,
-                  _lib.stream_ptr(dev))
+                  pointers(*target), words(*row), parents.data_ptr(), B, k, K, _lib.stream_ptr(dev))
     return out[0] if one else out

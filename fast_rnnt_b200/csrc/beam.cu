@@ -523,36 +523,53 @@ select_join_kernel(const SelSum *__restrict__ sums, const uint64_t *__restrict__
   }
 }
 
-// ------------------------------------------------------------------------------
+// ---- reordering --------------------------------------------------------------------------
+// A gather of rows, bound by memory: every thread has several pieces of 16 bytes (or fewer, where
+// rows do not begin on such boundaries) under way at once, since each waits for its parent first.
 constexpr int kReorderMost = 32;   // tensors of one launch
+constexpr int kReorderThreads = 256, kReorderPieces = 4;
 struct ReorderList {
   const char *from[kReorderMost];
   char *to[kReorderMost];
   long long batch[kReorderMost], beam[kReorderMost];   // strides of `from` in bytes
   long long bytes[kReorderMost];                       // of one row
+  int width[kReorderMost];                             // of a piece
 };
 
 template <typename W>
-__device__ __forceinline__ void copy_row(const char *from, char *to, long long bytes) {
-  for (long long n = threadIdx.x; n < bytes / (long long)sizeof(W); n += blockDim.x)
-    reinterpret_cast<W *>(to)[n] = from == nullptr ? W{} : reinterpret_cast<const W *>(from)[n];
+__device__ __forceinline__ void reorder_pieces(const ReorderList &list, int n, const int64_t *__restrict__ parents,
+                                               long long rows, int beams, int K) {
+  const long long per = list.bytes[n] / (long long)sizeof(W), all = rows * per;
+  const long long first = (long long)blockIdx.x * (kReorderThreads * kReorderPieces) + threadIdx.x;
+  W piece[kReorderPieces];
+#pragma unroll
+  for (int u = 0; u < kReorderPieces; ++u) {
+    const long long at = first + u * kReorderThreads;
+    if (at >= all) break;
+    const long long row = all <= INT_MAX ? (int)at / (int)per : at / per;
+    const int64_t p = parents[row];
+    piece[u] = W{};
+    if (p >= 0 && p < K)
+      piece[u] = __ldg(reinterpret_cast<const W *>(list.from[n] + div_rows(row, beams) * list.batch[n] +
+                                                   p * list.beam[n]) + (at - row * per));
+  }
+#pragma unroll
+  for (int u = 0; u < kReorderPieces; ++u) {
+    const long long at = first + u * kReorderThreads;
+    if (at < all) reinterpret_cast<W *>(list.to[n])[at] = piece[u];
+  }
 }
 
-__global__ void __launch_bounds__(128)
+__global__ void __launch_bounds__(kReorderThreads)
 beam_reorder_kernel(const __grid_constant__ ReorderList list, const int64_t *__restrict__ parents, long long rows,
                     int beams, int K) {
   const int n = blockIdx.y;
-  const long long bytes = list.bytes[n];
-  for (long long row = blockIdx.x; row < rows; row += gridDim.x) {
-    const int64_t p = parents[row];
-    const char *from = p < 0 || p >= K ? nullptr
-                                       : list.from[n] + div_rows(row, beams) * list.batch[n] + p * list.beam[n];
-    char *to = list.to[n] + row * bytes;
-    const uintptr_t low = (uintptr_t)from | (uintptr_t)to | (uintptr_t)bytes;
-    if (low % 16 == 0) copy_row<uint4>(from, to, bytes);
-    else if (low % 4 == 0) copy_row<uint32_t>(from, to, bytes);
-    else if (low % 2 == 0) copy_row<uint16_t>(from, to, bytes);
-    else copy_row<uint8_t>(from, to, bytes);
+  switch (list.width[n]) {
+    case 16: reorder_pieces<uint4>(list, n, parents, rows, beams, K); break;
+    case 8: reorder_pieces<uint2>(list, n, parents, rows, beams, K); break;
+    case 4: reorder_pieces<uint32_t>(list, n, parents, rows, beams, K); break;
+    case 2: reorder_pieces<uint16_t>(list, n, parents, rows, beams, K); break;
+    default: reorder_pieces<uint8_t>(list, n, parents, rows, beams, K);
   }
 }
 
@@ -637,15 +654,22 @@ extern "C" int frnnt_beam_reorder(int count, const void *const *from, const long
   for (int first = 0; first < count; first += kReorderMost) {
     ReorderList list{};
     const int m = count - first < kReorderMost ? count - first : kReorderMost;
+    long long blocks = 1;
     for (int n = 0; n < m; ++n) {
       list.from[n] = (const char *)from[first + n];
       list.to[n] = (char *)to[first + n];
       list.batch[n] = batch[first + n];
       list.beam[n] = beam[first + n];
       list.bytes[n] = bytes[first + n];
+      const unsigned long long low = (uintptr_t)list.from[n] | (uintptr_t)list.to[n] | (unsigned long long)list.batch[n] |
+                                     (unsigned long long)list.beam[n] | (unsigned long long)list.bytes[n];
+      list.width[n] = low % 16 == 0 ? 16 : low % 8 == 0 ? 8 : low % 4 == 0 ? 4 : low % 2 == 0 ? 2 : 1;
+      const long long pieces = rows * (list.bytes[n] / list.width[n]);
+      const long long need = (pieces + kReorderThreads * kReorderPieces - 1) / (kReorderThreads * kReorderPieces);
+      blocks = need > blocks ? need : blocks;
     }
-    const long long most = (long long)sm_count() * 64;
-    FRNNT_KERNEL(beam_reorder_kernel<<<dim3((unsigned)(rows < most ? rows : most), (unsigned)m), 128, 0, st>>>(
+    FRNNT_REQUIRE(blocks <= INT_MAX, FRNNT_EUNSUPPORTED, "too many rows for the grid");
+    FRNNT_KERNEL(beam_reorder_kernel<<<dim3((unsigned)blocks, (unsigned)m), kReorderThreads, 0, st>>>(
         list, parents, rows, beams, K));
     FRNNT_CUDA(cudaGetLastError());
   }

@@ -515,31 +515,53 @@ recurrence_backward_kernel(RecTensor x, RecTensor gate, const int64_t *__restric
   if constexpr (CLUSTER) mail_end(mail);
 }
 
-constexpr int kStepThreads = 128;
-
 // One token: every row reads the state of its parent (its own without parents; zero where the
-// parent is not one of the K rows) and writes the new state and its rounding to x's type.
-template <typename T>
+// parent is not one of the K rows) and writes the new state and its rounding to x's type.  A
+// thread has VEC channels: 16 bytes of x and of gate where all rows allow that.
+constexpr int kStepThreads = 256;
+
+template <typename T, int VEC>
 __global__ void __launch_bounds__(kStepThreads)
 recurrence_step_kernel(const T *__restrict__ x, long long x_row, const T *__restrict__ gate, long long gate_row,
                        const RecState<T> *__restrict__ state, const int64_t *__restrict__ parents,
                        T *__restrict__ h, RecState<T> *__restrict__ next, long long rows, int beams, int K, int D) {
   using real = RecState<T>;
-  const int d = blockIdx.x * kStepThreads + threadIdx.x;
-  if (d >= D) return;
-  for (long long row = blockIdx.y; row < rows; row += gridDim.y) {
-    long long from = row;
-    if (parents != nullptr) {
-      const int64_t p = parents[row];
-      from = p < 0 || p >= K ? -1 : div_rows(row, beams) * K + p;
-    }
-    real keep, take;
-    gate_pair<T>(rec_value<T>(gate[row * gate_row + d]), keep, take);
-    const real old = from < 0 ? real(0) : state[from * D + d];
-    const real now = keep * old + take * rec_value<T>(x[row * x_row + d]);
-    next[row * D + d] = now;
-    if (h != nullptr) h[row * D + d] = rec_round<T>(now);
+  using Pack = RecPack<T, VEC>;
+  const int per = D / VEC;
+  const long long n = (long long)blockIdx.x * kStepThreads + threadIdx.x, row = div_rows(n, per);
+  if (row >= rows) return;
+  const int d = (int)(n - row * per) * VEC;
+  const Pack xp = *reinterpret_cast<const Pack *>(x + row * x_row + d);
+  const Pack gp = *reinterpret_cast<const Pack *>(gate + row * gate_row + d);
+  long long from = row;
+  if (parents != nullptr) {
+    const int64_t p = parents[row];
+    from = p < 0 || p >= K ? -1 : div_rows(row, beams) * K + p;
   }
+  real xv[VEC], gv[VEC], old[VEC], take[VEC], keep[VEC];
+  if (from >= 0) get<real, VEC>(state + from * D + d, old);
+  else vset(old, real(0));
+  rec_unpack<T, VEC>(xp, xv);
+  rec_unpack<T, VEC>(gp, gv);
+#pragma unroll
+  for (int k = 0; k < VEC; ++k) gate_pair<T>(gv[k], keep[k], take[k]);
+  vmul(xv, take, xv);
+  vfma(old, keep, old, xv);
+  put<real, VEC>(next + row * D + d, old);
+  if (h != nullptr) *reinterpret_cast<Pack *>(h + row * D + d) = rec_pack<T, VEC>(old);
+}
+
+template <typename T, int VEC>
+static int step_as(const void *x, long long x_row, const void *gate, long long gate_row, const void *state,
+                   const int64_t *parents, void *h, void *next, long long rows, int beams, int K, int D,
+                   cudaStream_t st) {
+  const long long blocks = (rows * (D / VEC) + kStepThreads - 1) / kStepThreads;
+  FRNNT_REQUIRE(blocks <= INT_MAX, FRNNT_EUNSUPPORTED, "too many rows for the grid");
+  FRNNT_KERNEL(recurrence_step_kernel<T, VEC><<<(unsigned)blocks, kStepThreads, 0, st>>>(
+      (const T *)x, x_row, (const T *)gate, gate_row, (const RecState<T> *)state, parents, (T *)h,
+      (RecState<T> *)next, rows, beams, K, D));
+  FRNNT_CUDA(cudaGetLastError());
+  return FRNNT_OK;
 }
 
 // ---- host ----------------------------------------------------------------------------
@@ -548,7 +570,7 @@ recurrence_step_kernel(const T *__restrict__ x, long long x_row, const T *__rest
 // multiprocessor a CTA, no more than the sequence has.
 static int ranks_for(long long ctas, int T) {
   int ranks = 1;
-  while (ranks < kRecMostCluster && ctas * ranks < 3 * sm_count() && 2 * ranks <= (T + kRecChunk - 1) / kRecChunk)
+  while (ranks < kRecMostCluster && ctas * ranks * 2 <= 3 * sm_count() && 2 * ranks <= (T + kRecChunk - 1) / kRecChunk)
     ranks *= 2;
   return ranks;
 }
@@ -633,14 +655,6 @@ static int backward_as(const RecTensor &x, const RecTensor &gate, const int64_t 
 
 using namespace frnnt;
 
-#define FRNNT_REC_TYPES(CALL) \
-  switch (dtype) {            \
-    case FRNNT_F32: CALL(float); break;           \
-    case FRNNT_F64: CALL(double); break;          \
-    case FRNNT_F16: CALL(__half); break;          \
-    default: CALL(__nv_bfloat16); break;          \
-  }
-
 static bool rec_dtype(int dtype) {
   return dtype == FRNNT_F32 || dtype == FRNNT_F64 || dtype == FRNNT_F16 || dtype == FRNNT_BF16;
 }
@@ -704,14 +718,17 @@ extern "C" int frnnt_recurrence_step(int dtype, const void *x, long long x_row, 
   if (rows == 0 || D == 0) return FRNNT_OK;
   FRNNT_REQUIRE(x && gate && state && next, FRNNT_EINVAL, "NULL argument");
   FRNNT_REQUIRE(state != next, FRNNT_EINVAL, "the new states may not overwrite the old ones");
-  cudaStream_t st = (cudaStream_t)stream;
-  const dim3 grid((unsigned)((D + kStepThreads - 1) / kStepThreads), (unsigned)(rows < 65535 ? rows : 65535));
-#define FRNNT_REC_STEP(TYPE)                                                                \
-  FRNNT_KERNEL(recurrence_step_kernel<TYPE><<<grid, kStepThreads, 0, st>>>(                  \
-      (const TYPE *)x, x_row, (const TYPE *)gate, gate_row, (const RecState<TYPE> *)state,  \
-      parents, (TYPE *)h, (RecState<TYPE> *)next, rows, beams, K, D))
-  FRNNT_REC_TYPES(FRNNT_REC_STEP)
+  const int size = rec_size(dtype);
+  const auto aligned = [&](const void *p, long long row) { return (uintptr_t)p % 16 == 0 && row * size % 16 == 0; };
+  const bool wide = aligned(x, x_row) && aligned(gate, gate_row) && aligned(h, D) && (uintptr_t)state % 16 == 0 &&
+                    (uintptr_t)next % 16 == 0;   // rows of states are as wide or wider
+#define FRNNT_REC_STEP(TYPE, VEC) \
+  step_as<TYPE, VEC>(x, x_row, gate, gate_row, state, parents, h, next, rows, beams, K, D, (cudaStream_t)stream)
+  switch (dtype) {
+    case FRNNT_F32: return wide ? FRNNT_REC_STEP(float, 4) : FRNNT_REC_STEP(float, 1);
+    case FRNNT_F64: return wide ? FRNNT_REC_STEP(double, 2) : FRNNT_REC_STEP(double, 1);
+    case FRNNT_F16: return wide ? FRNNT_REC_STEP(__half, 8) : FRNNT_REC_STEP(__half, 1);
+    default: return wide ? FRNNT_REC_STEP(__nv_bfloat16, 8) : FRNNT_REC_STEP(__nv_bfloat16, 1);
+  }
 #undef FRNNT_REC_STEP
-  FRNNT_CUDA(cudaGetLastError());
-  return FRNNT_OK;
 }
