@@ -53,12 +53,23 @@ class GraphedStep:
                                                          if isinstance(v, Tensor) and v.requires_grad]
         for k in names:
             inputs[k].grad = None
+        # leaves of the capture's own over the same memory: an eager graph of the caller's leaves that
+        # is still alive holds their gradient accumulators on its own stream, which a capture
+        # cannot wait for
+        own = {k: v.detach().requires_grad_(True) if k in names and v.is_leaf else v
+               for k, v in inputs.items()}
         torch.cuda.synchronize(dev)
         torch.cuda.empty_cache()   # the warm-up's scratch, or it stays cached beside the graph's
         n0 = _lib.lib().frnnt_launch_count()
         with torch.cuda.graph(self.graph, pool=pool):
-            self.loss = fn(inputs)
+            self.loss = fn(own)
         self.launches = int(_lib.lib().frnnt_launch_count() - n0)
+        for k, v in own.items():
+            if v is not inputs.get(k):
+                if k in inputs:
+                    inputs[k].grad = v.grad
+                else:
+                    inputs[k] = v   # what `fn` put there
 
     def __call__(self) -> Tensor:
         self.graph.replay()
