@@ -55,8 +55,8 @@ def beam_select(logits: Tensor, scores: Tensor, beam: int, termination_symbol: i
     scores = scores.contiguous()
     code, (sb, sk, _) = _lib.input_code(logits.dtype), logits.stride()
     with _lib.on_device(dev):
-        best = scores.new_empty((B, beam))
-        parents = scores.new_empty((B, beam), dtype=torch.int64)
+        best = torch.empty_like(scores) if beam == K else scores.new_empty((B, beam))
+        parents = torch.empty_like(best, dtype=torch.int64)
         tokens = torch.empty_like(parents)
         n = _lib.size_of("frnnt_beam_select_scratch_bytes", code, B, K, V, beam)
         scratch = scores.new_empty(n, dtype=torch.uint8)
