@@ -33,7 +33,7 @@ def beam_select(logits: Tensor, scores: Tensor, beam: int, termination_symbol: i
     left, the slots behind them hold a score of -inf and -1 as parent and token, which
     beam_reorder and gated_recurrence_step take as no hypothesis.
 
-    K is at most 1024, beam at most 32.  Not differentiable."""
+    B is at most 65535, K at most 1024, beam at most 32.  Not differentiable."""
     assert logits.ndim == 3, logits.ndim
     (B, K, V) = logits.shape
     assert K >= 1 and V >= 1, logits.shape

@@ -93,14 +93,19 @@ template <typename T> struct SelRow {
   }
   // whole 32-bit words that the row begins behind a boundary; -1: on one
   __device__ __forceinline__ int words() const { return off == 0 ? -1 : off * (int)sizeof(T) / 4; }
-  template <int W> __device__ __forceinline__ uint4 load(int j) const {
+  struct Raw {
+    uint4 q, r;   // a vector's granule and, off a boundary, the next one
+  };
+  template <int W> __device__ __forceinline__ Raw load(int j) const {
     const uint4 *p = reinterpret_cast<const uint4 *>(row - off) + j;
-    const uint4 q = __ldg(p);
+    if constexpr (W < 0) return {__ldg(p), {}};
+    else return {__ldg(p), __ldg(p + 1)};
+  }
+  template <int W> __device__ __forceinline__ uint4 vector_of(const Raw &raw) const {
     if constexpr (W < 0) {
-      return q;
+      return raw.q;
     } else {
-      const uint4 r = __ldg(p + 1);
-      const uint32_t w[8] = {q.x, q.y, q.z, q.w, r.x, r.y, r.z, r.w};
+      const uint32_t w[8] = {raw.q.x, raw.q.y, raw.q.z, raw.q.w, raw.r.x, raw.r.y, raw.r.z, raw.r.w};
       if constexpr (sizeof(T) == 4) return make_uint4(w[W], w[W + 1], w[W + 2], w[W + 3]);
       else
         return make_uint4(__funnelshift_r(w[W], w[W + 1], half), __funnelshift_r(w[W + 1], w[W + 2], half),
@@ -202,12 +207,20 @@ struct SelShare {
 template <typename T, int W>
 __device__ __forceinline__ void stream_row(SelShare &own, const SelRow<T> &row, int first, int end, bool read) {
   constexpr int EV = SelRow<T>::EV, U = 2;
-  for (int j = first + (int)threadIdx.x; j < end; j += U * kSelThreads) {
-    uint4 q[U];
+  typename SelRow<T>::Raw ahead[U];
+  const auto fetch = [&](int j) {
 #pragma unroll
     for (int n = 0; n < U; ++n)
-      if (j + n * kSelThreads < end) q[n] = row.template load<W>(j + n * kSelThreads);
-    if (!read) return;
+      if (j + n * kSelThreads < end) ahead[n] = row.template load<W>(j + n * kSelThreads);
+  };
+  int j = first + (int)threadIdx.x;
+  fetch(j);
+  if (!read) return;
+  for (; j < end; j += U * kSelThreads) {
+    uint4 q[U];
+#pragma unroll
+    for (int n = 0; n < U; ++n) q[n] = row.template vector_of<W>(ahead[n]);
+    fetch(j + U * kSelThreads);
 #pragma unroll
     for (int n = 0; n < U; ++n)
       if (j + n * kSelThreads < end) {

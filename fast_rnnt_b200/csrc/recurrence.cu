@@ -14,9 +14,13 @@
 // same products of gates.  h_{t-1} is recomputed from the state that the forward keeps per tile:
 // 5 values an element move instead of 6, and h keeps its 32 bits.
 //
-// Both are bound by memory: 3 values an element forward, 5 backward, in their own type.  Inputs
-// go to shared memory with cp.async a tile ahead, each thread fetching just what it reads
-// itself, so that no barrier belongs to the copies.
+// Both are bound by memory where there are channels enough: 3 values an element forward, 5
+// backward, in their own type (64 x 500 x 2048 bf16, ragged: 67 and 115 us, 0.9 of the copy rate
+// if nothing were padding).  Inputs go to shared memory with cp.async a tile ahead, each thread
+// fetching just what it reads itself, so that no barrier belongs to the copies.  Tiles of 32
+// channels and 128 threads, four CTAs a multiprocessor forward and three backward, took the place
+// of 64 channels and 256 threads (16 x 2000 x 1024 bf16: 47 + 85 -> 38 + 71 us); the backward
+// then issues an instruction in two cycles of three, its products and sums two floats at a time.
 #include <cooperative_groups.h>
 
 #include <atomic>
@@ -566,8 +570,11 @@ static int step_as(const void *x, long long x_row, const void *gate, long long g
 
 // ---- host ----------------------------------------------------------------------------
 
-// CTAs of a cluster: as many tiles of one sequence at once as it takes to give every
-// multiprocessor a CTA, no more than the sequence has.
+// CTAs of a cluster: tiles of one sequence at once, doubled as long as the whole grid still fits the
+// three CTAs that a multiprocessor holds (a second turn of the grid costs more than the idle
+// multiprocessors: 1 x 8000 x 1024 bf16, 512 of 444 places 25 + 45 us, 256 of them 20 + 27), no
+// more than the sequence has.  One long sequence of few channels gets 16 (1 x 30011 x 512 fp16:
+// 40 us, with 8 CTAs 55, without a cluster 8 CTAs in all).
 static int ranks_for(long long ctas, int T) {
   int ranks = 1;
   while (ranks < kRecMostCluster && ctas * ranks * 2 <= 3 * sm_count() && 2 * ranks <= (T + kRecChunk - 1) / kRecChunk)
@@ -580,7 +587,7 @@ static int rec_launch(void (*alone)(Params...), void (*cluster)(Params...), int 
                       cudaStream_t st, Args... args) {
   const int tiles = (D + S::kWidth - 1) / S::kWidth;
   FRNNT_REQUIRE(B <= 65535 && tiles <= 65535, FRNNT_EUNSUPPORTED, "B or D too large for the grid");
-  FRNNT_REQUIRE(T <= INT_MAX - kRecMostCluster * kRecChunk, FRNNT_EUNSUPPORTED, "T too large");
+  FRNNT_REQUIRE(T <= INT_MAX - 4 * kRecMostCluster * kRecChunk, FRNNT_EUNSUPPORTED, "T too large");
   const int ranks = ranks_for((long long)B * tiles, T);
   const size_t smem = 2 * (size_t)arrays * (S::kStage + S::kExchange * sizeof(typename S::real)) +
                       (ranks > 1 ? 4 * ranks * S::kWidth * sizeof(typename S::real) + 16 : 0);

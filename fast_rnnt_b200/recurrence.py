@@ -104,7 +104,8 @@ def gated_recurrence(x: Tensor, gate: Tensor, initial: Optional[Tensor] = None,
     which is initial[b] for an empty sequence.  Lengths below 0 or above T count as 0 and T.
     A gate of -inf drops the state (h[:, t] = x[:, t]) and one of +inf keeps it.
 
-    Differentiable once with respect to x, gate and initial.  No counterpart in the reference."""
+    B is at most 65535.  A sequence has the same bits in any batch.  Differentiable once with
+    respect to x, gate and initial.  No counterpart in the reference."""
     assert x.ndim == 3, x.ndim
     shape, dtype, dev = x.shape, x.dtype, x.device
     assert gate.shape == shape, (gate.shape, shape)

@@ -159,6 +159,17 @@ def test_without_gradients_the_same_bits_and_twice_the_same():
     assert torch.equal(h, a["h"]) and torch.equal(last, a["last"])
 
 
+@pytest.mark.parametrize("T", [100, 700, 2300])
+def test_a_sequence_alone_has_the_bits_it_has_in_a_batch(T):
+    """However many tiles of it are taken at once."""
+    x, gate, m = make(40, T, 96, torch.float32, seed=19)
+    batch = run(x, gate, **m)
+    for b in (0, 39):
+        alone = run(x[b:b + 1], gate[b:b + 1], **{k: v[b:b + 1] for k, v in m.items()})
+        for name in alone:
+            assert torch.equal(alone[name][0], batch[name][b]), name
+
+
 def test_state_carried_between_pieces():
     """A sequence in pieces, each from the state of the one before, as a streaming encoder runs."""
     import fast_rnnt_b200 as fr
