@@ -54,18 +54,24 @@ template <int LEFT> __device__ __forceinline__ void copy_wait() {
 template <typename S> struct RecTile {
   using T = typename S::T;
   using Pack = RecPack<T, S::VEC>;
-  __device__ static void fetch(Pack *tile, const T *from, long long step, int first, int n, const Pack &pad) {
+  __device__ static __forceinline__ void fetch(Pack *tile, const T *from, long long step, int first, int n,
+                                               const Pack &pad) {
+    const T *p = from + first * step;
+    if constexpr (sizeof(Pack) == 2) {   // all loads under way before the first is stored
+      Pack v[S::kSteps];
 #pragma unroll
-    for (int s = 0; s < S::kSteps; ++s) {
-      if (first + s >= n) {
-        tile[s * kRecThreads] = pad;
-        continue;
+      for (int s = 0; s < S::kSteps; ++s, p += step) v[s] = first + s < n ? *reinterpret_cast<const Pack *>(p) : pad;
+#pragma unroll
+      for (int s = 0; s < S::kSteps; ++s) tile[s * kRecThreads] = v[s];
+    } else if (first + S::kSteps <= n) {   // nearly always: no comparisons per step
+#pragma unroll
+      for (int s = 0; s < S::kSteps; ++s, p += step) copy_async<(int)sizeof(Pack)>(&tile[s * kRecThreads], p);
+    } else {
+#pragma unroll
+      for (int s = 0; s < S::kSteps; ++s, p += step) {
+        if (first + s < n) copy_async<(int)sizeof(Pack)>(&tile[s * kRecThreads], p);
+        else tile[s * kRecThreads] = pad;
       }
-      const T *p = from + (first + s) * step;
-      if constexpr (sizeof(Pack) == 2)
-        tile[s * kRecThreads] = *reinterpret_cast<const Pack *>(p);
-      else
-        copy_async<(int)sizeof(Pack)>(&tile[s * kRecThreads], p);
     }
   }
 };
@@ -326,11 +332,19 @@ recurrence_forward_kernel(RecTensor x, RecTensor gate, const typename S::real *_
     __syncthreads();
     real state[VEC];
     get<real, VEC>(EB + S::at(at.piece, at.c), state);
+    T *out = H + (size_t)first * D;
+    if (first + STEPS <= here) {   // nearly always
 #pragma unroll
-    for (int s = 0; s < STEPS; ++s) {
-      vfma(state, f[s], state, u[s]);
-      if (first + s < here)
-        *reinterpret_cast<Pack *>(H + (size_t)(first + s) * D) = rec_pack<T, VEC>(state);
+      for (int s = 0; s < STEPS; ++s, out += D) {
+        vfma(state, f[s], state, u[s]);
+        *reinterpret_cast<Pack *>(out) = rec_pack<T, VEC>(state);
+      }
+    } else {
+#pragma unroll
+      for (int s = 0; s < STEPS; ++s, out += D) {
+        vfma(state, f[s], state, u[s]);
+        if (first + s < here) *reinterpret_cast<Pack *>(out) = rec_pack<T, VEC>(state);
+      }
     }
   }
   if (at.inside) {   // behind the sequence
@@ -389,7 +403,7 @@ recurrence_backward_kernel(RecTensor x, RecTensor gate, const int64_t *__restric
     if constexpr (!CLUSTER) fetch(turn - 1);
     const int chunk = turn * ranks + rank, first = chunk * kRecChunk + piece_first;
     real start = real(0);   // the state before the tile
-    if (keeper && chunk * kRecChunk < n) start = saved[((size_t)b * chunks + chunk) * D + join_channel];
+    if (keeper && saved != nullptr && chunk * kRecChunk < n) start = saved[((size_t)b * chunks + chunk) * D + join_channel];
     copy_wait<CLUSTER ? 0 : 1>();
     real *const EA = exchange + (turn & 1) * 3 * S::kExchange, *const EB = EA + S::kExchange,
                *const EM = EB + S::kExchange;
@@ -494,9 +508,9 @@ recurrence_backward_kernel(RecTensor x, RecTensor gate, const int64_t *__restric
       vmul(u, take[s], xv);
       vfma(state, f[s], state, u);
     }
-#pragma unroll
-    for (int s = STEPS - 1; s >= 0; --s) {
-      if (first + s >= here) continue;
+    const size_t behind = (size_t)(first + STEPS) * D;
+    T *out_x = DX + behind, *out_g = DG + behind;
+    const auto step_back = [&](int s, bool live) {
       real dv[VEC], lam[VEC], ox[VEC], og[VEC];
       rec_unpack<T, VEC>(tile[(2 * STEPS + s) * kRecThreads], dv);
       vadd(lam, back, dv);
@@ -504,8 +518,19 @@ recurrence_backward_kernel(RecTensor x, RecTensor gate, const int64_t *__restric
       vmul(ox, take[s], lam);
       vmul(og, before[s], take[s]);
       vmul(og, og, back);           // lam (h - x) f take
-      *reinterpret_cast<Pack *>(DX + (size_t)(first + s) * D) = rec_pack<T, VEC>(ox);
-      *reinterpret_cast<Pack *>(DG + (size_t)(first + s) * D) = rec_pack<T, VEC>(og);
+      out_x -= D;
+      out_g -= D;
+      if (live) {
+        *reinterpret_cast<Pack *>(out_x) = rec_pack<T, VEC>(ox);
+        *reinterpret_cast<Pack *>(out_g) = rec_pack<T, VEC>(og);
+      }
+    };
+    if (first + STEPS <= here) {   // nearly always
+#pragma unroll
+      for (int s = STEPS - 1; s >= 0; --s) step_back(s, true);
+    } else {
+#pragma unroll
+      for (int s = STEPS - 1; s >= 0; --s) step_back(s, first + s < here);
     }
   }
   if (at.inside) {   // behind the sequence
@@ -669,7 +694,7 @@ static int rec_size(int dtype) { return dtype == FRNNT_F64 ? 8 : dtype == FRNNT_
 static bool rec_sizes(int B, int T, int D) { return B >= 0 && T >= 0 && D >= 0; }
 
 extern "C" size_t frnnt_recurrence_saved_bytes(int dtype, int B, int T, int D) {
-  if (!rec_dtype(dtype) || B <= 0 || T <= 0 || D <= 0) return 0;
+  if (!rec_dtype(dtype) || B <= 0 || T <= kRecChunk || D <= 0) return 0;   // one tile starts from `initial`
   return (size_t)B * ((T + kRecChunk - 1) / kRecChunk) * D * (dtype == FRNNT_F64 ? 8 : 4);
 }
 
@@ -701,7 +726,7 @@ extern "C" int frnnt_recurrence_backward(int dtype, const void *x, long long x_b
   FRNNT_REQUIRE(rec_dtype(dtype), FRNNT_EINVAL, "dtype must be FRNNT_F32, _F64, _F16 or _BF16");
   FRNNT_REQUIRE(rec_sizes(B, T, D), FRNNT_EINVAL, "bad sizes");
   if (B == 0 || D == 0) return FRNNT_OK;
-  FRNNT_REQUIRE(T == 0 || (x && gate && saved && dx && dgate), FRNNT_EINVAL, "NULL argument");
+  FRNNT_REQUIRE(T == 0 || (x && gate && (saved || T <= kRecChunk) && dx && dgate), FRNNT_EINVAL, "NULL argument");
   const RecTensor X{x, x_batch, x_step}, G{gate, gate_batch, gate_step}, DH{dh, dh_batch, dh_step};
   const int size = rec_size(dtype);
   const auto fits = [&](int bytes) {

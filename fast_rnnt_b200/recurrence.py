@@ -39,12 +39,13 @@ def _forward(x, gate, initial, lengths, keep_states):
         last = x.new_empty((B, D), dtype=_state_type(x.dtype))
         if keep_states:
             n = _lib.size_of("frnnt_recurrence_saved_bytes", code, B, T, D)
-            saved = x.new_empty(n, dtype=torch.uint8)
+            saved = x.new_empty(n, dtype=torch.uint8) if n else initial   # none: a short sequence
         xs, gs = x.stride(), gate.stride()
         _lib.call("frnnt_recurrence_forward", code, x.data_ptr(), xs[0], xs[1], gate.data_ptr(), gs[0],
                   gs[1], None if initial is None else initial.data_ptr(),
                   None if lengths is None else lengths.data_ptr(), h.data_ptr(), last.data_ptr(),
-                  None if saved is None else saved.data_ptr(), B, T, D, _lib.stream_ptr(dev))
+                  None if saved is None or saved is initial else saved.data_ptr(), B, T, D,
+                  _lib.stream_ptr(dev))
     return h, last, saved
 
 
@@ -63,7 +64,8 @@ def _backward(ctx, dh, dlast):
                     if ctx.needs_input_grad[2] else None)
         xs, gs, ds = x.stride(), gate.stride(), (0, 0) if dh is None else dh.stride()
         _lib.call("frnnt_recurrence_backward", code, x.data_ptr(), xs[0], xs[1], gate.data_ptr(), gs[0],
-                  gs[1], None if lengths is None else lengths.data_ptr(), saved.data_ptr(),
+                  gs[1], None if lengths is None else lengths.data_ptr(),
+                  None if saved is None else saved.data_ptr(),
                   None if dh is None else dh.data_ptr(), ds[0], ds[1],
                   None if dlast is None else dlast.data_ptr(), dx.data_ptr(), dgate.data_ptr(),
                   None if dinitial is None else dinitial.data_ptr(), B, T, D, _lib.stream_ptr(dev))

@@ -430,7 +430,8 @@ int frnnt_pair_matmul_tn(const void *a_hi, const void *a_lo, const void *b_hi, c
  * everywhere) counts the steps of each sequence (below 0: 0, above T: T): the steps behind them
  * are not read, h is zero there, and last is the state after the last step that counts.
  * saved (NULL when no backward follows; frnnt_recurrence_saved_bytes) receives the states from
- * which the backward recomputes h. */
+ * which the backward recomputes h.  Up to 128 steps that is `initial` itself: the size is 0 and
+ * the backward takes `initial`, or NULL, in its place. */
 size_t frnnt_recurrence_saved_bytes(int dtype, int B, int T, int D);
 int frnnt_recurrence_forward(int dtype, const void *x, long long x_batch, long long x_step, const void *gate,
                              long long gate_batch, long long gate_step, const void *initial,

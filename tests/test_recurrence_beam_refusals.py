@@ -65,7 +65,7 @@ def test_c_abi_checks(fr):
     refused(*seq(0, 1, 1, 1, None), text=b"NULL")
     assert lib.frnnt_recurrence_forward(*seq(0, 0, 5, 5)[1:]) == 0
     back = lambda dtype, saved: ("frnnt_recurrence_backward", dtype, one, n(0), n(0), one, n(0), n(0), None, saved,  # noqa: E731
-                                 None, n(0), n(0), None, one, one, None, 1, 4, 4, None)
+                                 None, n(0), n(0), None, one, one, None, 1, 400, 4, None)
     refused(*back(-1, one), text=b"dtype")
     refused(*back(0, None), text=b"NULL")
     refused("frnnt_recurrence_step", 0, one, n(4), one, n(4), one, None, None, one, n(2), 1, 1, 4, None,
