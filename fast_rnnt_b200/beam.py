@@ -36,6 +36,7 @@ def beam_select(logits: Tensor, scores: Tensor, beam: int, termination_symbol: i
     B is at most 65535, K at most 1024, beam at most 32.  Not differentiable."""
     assert logits.ndim == 3, logits.ndim
     (B, K, V) = logits.shape
+    beam, termination_symbol = int(beam), int(termination_symbol)
     assert K >= 1 and V >= 1, logits.shape
     assert scores.shape == (B, K), (scores.shape, logits.shape)
     if logits.dtype != torch.float32 and not _lib.is_16bit(logits):

@@ -31,8 +31,9 @@
 namespace frnnt {
 
 // Small CTAs, many of them: a row's short phases after the stream run beside other rows' streams
-// (96 x 16 x 31999 fp16: 35 us; 256 threads, 5 CTAs a multiprocessor 39; 64 threads, 24 CTAs 48).
-constexpr int kSelThreads = 128, kSelResident = 12;
+// (96 x 16 x 31999 fp16: 34 us; 9 or 12 CTAs a multiprocessor 38 and 39, 256 threads and 5 CTAs 39,
+// 64 threads and 24 CTAs 48; reading the same bytes for their maxima alone takes 21 to 24).
+constexpr int kSelThreads = 128, kSelResident = 10;
 constexpr int kSelWarps = kSelThreads / 32;
 constexpr int kSelBeams = 1024;   // most rows of logits of one utterance
 constexpr int kSelMost = 32;      // most continuations
@@ -268,12 +269,82 @@ __device__ __forceinline__ int kind_of(float score, const uint8_t *finished, siz
   return !(fabsf(score) < INFINITY) ? 0 : finished != nullptr && finished[at] != 0 ? 1 : 2;
 }
 
+__device__ __forceinline__ void push_entry(RowShared &sm, uint64_t e) {
+  const int n = atomicAdd(&sm.found, 1);
+  if (n < kSelBuffer) sm.buffer[n] = e;
+}
+
+// `take` for every element of vector j that is `wanted`
+template <typename T, typename Wanted, typename Take>
+__device__ __forceinline__ void look_at(const SelRow<T> &row, int j, Wanted &&wanted, Take &&take) {
+  constexpr int EV = SelRow<T>::EV;
+  const uint4 q = load_any(row, j);
+  float x[EV];
+  SelRow<T>::unpack(q, x);
+  unsigned reach = 0;
+#pragma unroll
+  for (int e = 0; e < EV; ++e) reach |= (unsigned)wanted(x[e]) << e;
+  for (; reach != 0; reach &= reach - 1) {   // mostly one
+    const int at = __ffs(reach) - 1;
+    float v = x[0];
+#pragma unroll
+    for (int e = 1; e < EV; ++e) v = e == at ? x[e] : v;
+    take(entry_of(v, (uint32_t)(j * EV + at)));
+  }
+}
+
+// Where more reach the bound than the buffer holds: logits in clumps, or many equal ones.  The bound
+// again, the `beam`-th largest of all maxima now; what is above it lies in fewer than `beam`
+// columns, and of those equal to it only the lowest symbols count.  Returns how many it found,
+// still more than the buffer holds where the best ones lie in few columns.  Not inlined: it is
+// rare, and the registers it needs would be the kernel's.
+template <typename T>
+__device__ __noinline__ int crowded_row(RowShared &sm, SelRow<T> row, int first, int end, float top, float column_top,
+                                        float edge, int symbol, int beam) {
+  constexpr int EV = SelRow<T>::EV;
+  const int tid = threadIdx.x;
+  const uint32_t mine = ordered(top);
+  const auto push = [&](uint64_t e) { push_entry(sm, e); };
+  __syncthreads();   // all have seen how many there were
+  sm.column[tid] = (int)mine;
+  if (tid == 0) sm.found = 0;
+  __syncthreads();
+  int rank = 0;
+  for (int o = 0; o < kSelThreads; ++o) {
+    const uint32_t other = (uint32_t)sm.column[o];
+    rank += other > mine || (other == mine && o < tid);
+  }
+  if (rank == beam - 1) sm.bound[0] = mine;
+  __syncthreads();
+  const float bound = unordered(max(sm.bound[0], ordered(-FLT_MAX)));
+  const auto above = [&](float x) { return x > bound; };
+  const auto equal = [&](float x) { return x == bound; };
+  if (above(edge)) push(entry_of(edge, (uint32_t)symbol));
+  if (above(column_top))
+    for (int j = first + tid; j < end; j += kSelThreads) look_at(row, j, above, push);
+  __syncthreads();
+  // The lowest symbols: the first vector's, then some vectors at a time, no more than the buffer has
+  // room for, then the last two vectors'.  Everybody reads the count before anybody adds to it.
+  constexpr int kSome = (kSelBuffer - 4 * kSelMost) / EV;
+  int found = sm.found;
+  __syncthreads();
+  if (found < beam && equal(edge) && symbol < EV) push(entry_of(edge, (uint32_t)symbol));
+  for (int from = first; found < beam && from < end; from += kSome) {
+    for (int j = from + tid; j < min(end, from + kSome); j += kSelThreads) look_at(row, j, equal, push);
+    __syncthreads();
+    found = sm.found;
+    __syncthreads();
+  }
+  if (found < beam && equal(edge) && symbol >= EV) push(entry_of(edge, (uint32_t)symbol));
+  __syncthreads();
+  return sm.found;
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kSelThreads, kSelResident)
 select_rows_kernel(const T *__restrict__ logits, long long batch, long long row_stride,
                    const float *__restrict__ scores, const uint8_t *__restrict__ finished, int V,
                    SelSum *__restrict__ sums, uint64_t *__restrict__ entries, int beam) {
-  constexpr int EV = SelRow<T>::EV;
   __shared__ RowShared sm;
   // the second launch may be set up meanwhile; it waits for this one's end before it reads
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -330,28 +401,12 @@ select_rows_kernel(const T *__restrict__ logits, long long batch, long long row_
   for (int w = 0; w < kSelWarps; ++w) least = min(least, sm.bound[w]);
   const float bound = unordered(max(least, ordered(-FLT_MAX)));   // -inf is no candidate
   // collect
-  const auto push = [&](uint64_t e) {
-    const int n = atomicAdd(&sm.found, 1);
-    if (n < kSelBuffer) sm.buffer[n] = e;
-  };
-  const auto look = [&](int j, auto &&take) {
-    const uint4 q = load_any(row, j);
-    float x[EV];
-    SelRow<T>::unpack(q, x);
-    unsigned reach = 0;
-#pragma unroll
-    for (int e = 0; e < EV; ++e) reach |= (unsigned)(x[e] >= bound) << e;
-    for (; reach != 0; reach &= reach - 1) {   // mostly one
-      const int at = __ffs(reach) - 1;
-      float v = x[0];
-#pragma unroll
-      for (int e = 1; e < EV; ++e) v = e == at ? x[e] : v;
-      take(entry_of(v, (uint32_t)(j * EV + at)));
-    }
-  };
+  const auto push = [&](uint64_t e) { push_entry(sm, e); };
+  const auto look = [&](int j, auto &&wanted, auto &&take) { look_at(row, j, wanted, take); };
+  const auto reaches = [&](float x) { return x >= bound; };
   if (column_top >= bound) {
     if (column_next >= bound) sm.column[atomicAdd(&sm.columns, 1)] = tid;
-    else look(column_at, push);
+    else look(column_at, reaches, push);
   }
   if (edge >= bound) push(entry_of(edge, (uint32_t)symbol));
   if (warp == kSelWarps - 2 && lane < kSelWarps) {   // the row's maximum and sum
@@ -366,10 +421,12 @@ select_rows_kernel(const T *__restrict__ logits, long long batch, long long row_
   const int columns = sm.columns, pairs = columns * ((end - first + kSelThreads - 1) / kSelThreads);
   for (int p = tid; p < pairs; p += kSelThreads) {
     const int level = p / columns, j = first + sm.column[p - level * columns] + level * kSelThreads;
-    if (j < end) look(j, push);
+    if (j < end && *(volatile int *)&sm.found <= kSelBuffer) look(j, reaches, push);
   }
   if (columns > 0) __syncthreads();
-  const int found = sm.found;
+  int found = sm.found;
+  if (found > kSelBuffer)
+    found = crowded_row(sm, row, first, end, own.top, column_top, edge, symbol, beam);
   if (found <= kSelBuffer) {
     // order
     for (int c = tid; c < found; c += kSelThreads) {
@@ -380,14 +437,14 @@ select_rows_kernel(const T *__restrict__ logits, long long batch, long long row_
       if (earlier < beam) list[earlier] = mine;
     }
   } else {
-    // more than the buffer holds (equal logits, or the best ones in few columns): one at a time
+    // still more, where the best ones lie in few columns: one at a time
     uint64_t last = ~0ull;
     for (int n = 0; n < beam; ++n) {
       uint64_t best = 0;
       const auto keep = [&](uint64_t e) { best = e < last && e > best ? e : best; };
       if (edge >= bound) keep(entry_of(edge, (uint32_t)symbol));
       if (column_top >= bound)
-        for (int j = first + tid; j < end; j += kSelThreads) look(j, keep);
+        for (int j = first + tid; j < end; j += kSelThreads) look(j, reaches, keep);
       for (int o = 16; o > 0; o >>= 1) {
         const uint64_t other = __shfl_xor_sync(0xffffffffu, best, o);
         best = other > best ? other : best;

@@ -33,7 +33,11 @@ class GraphedStep:
     ``warmup`` eager runs on a side stream come first (lazy initialisation, the boundary cache,
     autograd's buffers), as torch's capture rules ask.  ``launches`` is the number of kernels of
     this library inside the graph.  ``pool`` (``torch.cuda.graph_pool_handle()``) lets several
-    captures that never run at the same time share their scratch memory."""
+    captures that never run at the same time share their scratch memory.
+
+    The capture runs on leaves of its own over the memory of those in ``inputs``, so that an eager
+    graph of the same leaves may still be alive (a loss that has not been released); leaves that
+    ``fn`` takes from elsewhere, a module's weights for instance, may not be part of one."""
 
     def __init__(self, fn: Callable[[Dict[str, Tensor]], Tensor], inputs: Dict[str, Tensor],
                  warmup: int = 3, leaves: Optional[Iterable[str]] = None, pool=None):

@@ -119,7 +119,7 @@ def gated_recurrence(x: Tensor, gate: Tensor, initial: Optional[Tensor] = None,
         assert initial.shape == (shape[0], shape[2]), (initial.shape, shape)
         assert initial.device == dev, (initial.device, dev)
         assert initial.dtype in (state, dtype), initial.dtype
-        initial = initial.to(state).contiguous()
+        initial = (initial if initial.dtype == state else initial.to(state)).contiguous()
     if lengths is not None:
         assert lengths.shape == shape[:1] and lengths.dtype == torch.int64, (lengths.shape, lengths.dtype)
         assert lengths.device == dev, (lengths.device, dev)

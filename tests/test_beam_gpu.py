@@ -74,6 +74,40 @@ def test_selection(B, K, V, beam, dtype):
     verify(logits, scores, beam)
 
 
+def test_most_hypotheses():
+    logits, scores = make(2, 1024, 65, "f32", seed=8)
+    verify(logits, scores, 32)
+    logits, scores = make(0, 3, 9, "f32")
+    import fast_rnnt_b200 as fr
+    assert [t.shape for t in fr.beam_select(logits, scores, 4)] == [(0, 4)] * 3
+
+
+def test_refusals():
+    import fast_rnnt_b200 as fr
+    logits, scores = make(2, 3, 40, "f32")
+    for beam in (0, 33):
+        with pytest.raises(fr.FrnntError, match="beam"):
+            fr.beam_select(logits, scores, beam)
+    many = torch.zeros(1, 1025, 4, device="cuda")
+    with pytest.raises(fr.FrnntError, match="beams"):
+        fr.beam_select(many, many[..., 0].contiguous(), 2)
+    for args in [(logits, scores.cpu(), 3), (logits.cpu(), scores, 3),
+                 (logits.clone().requires_grad_(True), scores, 3), (logits, scores.clone().requires_grad_(True), 3),
+                 (logits, scores, 3, 40, torch.zeros(2, 3, dtype=torch.bool, device="cuda")),
+                 (logits, scores, 3, 0, torch.zeros(2, 3, device="cuda")),
+                 (logits, scores, 3, 0, torch.zeros(2, 3, dtype=torch.bool))]:
+        with pytest.raises(AssertionError):
+            fr.beam_select(*args)
+    parents = torch.zeros(2, 4, dtype=torch.int64, device="cuda")
+    for states in ([logits, logits[:, :2]], [logits, logits[:1]], [logits.cpu()], [scores[0]],
+                   [logits.clone().requires_grad_(True)]):
+        with pytest.raises(AssertionError):
+            fr.beam_reorder(states, parents)
+    with torch.no_grad():    # gradients are not wanted: the same tensors are taken
+        fr.beam_reorder([logits.clone().requires_grad_(True)], parents)
+        fr.beam_select(logits.clone().requires_grad_(True), scores, 3)
+
+
 @pytest.mark.parametrize("dtype", list(TYPES))
 def test_dead_and_finished_hypotheses(dtype):
     logits, scores = make(6, 7, 333, dtype, seed=1)
@@ -140,6 +174,28 @@ def test_ties_go_to_the_lowest(V, dtype):
     s, p, t = fr.beam_select(rows, torch.zeros(1, 9, device="cuda"), 9)
     assert torch.equal(p[0].cpu(), torch.arange(9)), p
     assert (t == t[0, 0]).all() and (s == s[0, 0]).all()
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("V", [9, 300, 4233, 31999])
+def test_many_equal_logits(V, dtype):
+    """A few symbols allowed, the others masked by the lowest number; a plateau that begins late,
+    a plateau of every n-th symbol, and one behind all others."""
+    low = torch.finfo(TYPES[dtype]).min
+    n = torch.arange(V)
+    g = torch.Generator().manual_seed(V)
+    some = torch.randperm(V, generator=g)[:5]
+    x = torch.full((7, V), low, dtype=torch.float64)
+    x[0, some] = 1.5
+    x[1, some] = torch.randn(5, generator=g).double()
+    x[2] = torch.where(n > V // 2, 0.25, -1.0).double()
+    x[3] = torch.where(n % 611 == 7, 2.0, -2.0).double()
+    x[4] = torch.where(n >= V - 3, 3.0, 1.0).double()
+    x[5] = torch.where(n < 3, 3.0, 1.0).double()
+    x[6] = torch.where(n % 128 == 5, 4.0 + (n % 3) / 4, 1.0).double()
+    logits = x.to("cuda", TYPES[dtype])[:, None].repeat(1, 2, 1)
+    for beam in (1, 12, 32):
+        verify(logits, torch.zeros(7, 2, device="cuda"), beam)
 
 
 @pytest.mark.parametrize("dtype", list(TYPES))

@@ -183,6 +183,44 @@ def test_state_carried_between_pieces():
     check(state, want["last"], "last")
 
 
+def test_refusals():
+    import fast_rnnt_b200 as fr
+    x, gate, m = make(2, 5, 8, torch.float16)
+    lengths = torch.tensor([5, 5])
+    for args in [(x, gate.cpu()), (x, gate.float()), (x, gate, m["initial"].cpu()), (x, gate, m["initial"].double()),
+                 (x, gate, m["initial"][:1]), (x, gate, None, lengths), (x, gate, None, lengths.cuda().int()),
+                 (x, gate, None, lengths[:1].cuda())]:
+        with pytest.raises(AssertionError):
+            fr.gated_recurrence(*args)
+    state = m["initial"]
+    for args in [(x[:, 0], gate[:, 0], state.cpu()), (x[:, 0], gate[:, 0], state.half()),
+                 (x[:, 0], gate[:, 0], state.clone().requires_grad_(True)),
+                 (x, gate, state[:, None], torch.zeros(2, 5, dtype=torch.int64))]:
+        with pytest.raises(AssertionError):
+            fr.gated_recurrence_step(*args)
+    wide = torch.zeros(65536, 1, 1, device="cuda")
+    with pytest.raises(fr.FrnntError, match="too large"):
+        fr.gated_recurrence(wide, wide)
+
+
+def test_initial_state_changed_before_the_backward_pass():
+    """The state that gradients are computed from is the one of the forward pass, or an error."""
+    import fast_rnnt_b200 as fr
+    for T in (100, 300):
+        x, gate, m = make(2, T, 16, torch.float32, seed=20)
+        want = run(x, gate, m["initial"], dh=m["dh"])
+        leaf = x.clone().requires_grad_(True)
+        buffer = m["initial"].clone()
+        h, last = fr.gated_recurrence(leaf, gate, buffer)
+        buffer.zero_()
+        try:
+            (dx,) = torch.autograd.grad(h, leaf, m["dh"])
+        except RuntimeError as e:
+            assert "modified by an inplace operation" in str(e)
+        else:
+            assert torch.equal(dx, want["dx"])
+
+
 def test_second_derivative_is_refused():
     import fast_rnnt_b200 as fr
     x, gate, _ = make(1, 4, 4, torch.float32)
