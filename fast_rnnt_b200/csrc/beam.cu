@@ -31,8 +31,9 @@
 namespace frnnt {
 
 // Small CTAs, many of them: a row's short phases after the stream run beside other rows' streams
-// (96 x 16 x 31999 fp16: 34 us; 9 or 12 CTAs a multiprocessor 38 and 39, 256 threads and 5 CTAs 39,
-// 64 threads and 24 CTAs 48; reading the same bytes for their maxima alone takes 21 to 24).
+// (96 x 16 x 31999 fp16: 35 us; 12 CTAs a multiprocessor, with too few registers for that, 40, 256
+// threads and 5 CTAs 39, 64 threads and 24 CTAs 48; reading the same bytes for their maxima
+// alone takes 21 to 24).
 constexpr int kSelThreads = 128, kSelResident = 10;
 constexpr int kSelWarps = kSelThreads / 32;
 constexpr int kSelBeams = 1024;   // most rows of logits of one utterance
@@ -159,46 +160,39 @@ template <typename T> __device__ __forceinline__ uint4 load_any(const SelRow<T> 
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// What a thread keeps of its share of a row.  Exponents are taken to base 2, x log2(e) - R in one
-// multiply-add with R = ref log2(e) rounded, and `ref` follows the maximum only when that is far
-// above it: nearly every vector raises some lane's maximum, hardly one needs the sums rescaled.
-// Beyond 1e38, where the product would overflow (rows masked by the lowest number there is), and
-// before the first number, it is exp(x - ref) the long way.
+// What a thread keeps of its share of a row.  The sum of exponentials is relative to `ref`, which
+// follows the maximum only when that is far above it: nearly every vector raises some lane's
+// maximum, hardly one needs the sum rescaled.  All of it is arithmetic on differences of logits:
+// rows that differ by a constant (which the subtraction leaves exact) have equal sums.
 struct SelShare {
-  float top = neg_inf<float>(), next = neg_inf<float>(), ref = neg_inf<float>(), R = 0;
+  float top = neg_inf<float>(), next = neg_inf<float>(), ref = -FLT_MAX;
   float2 sum = {0, 0};
   int at = 0;   // the vector of `top`; `next` is the maximum of the others
-  static constexpr float kLog2e = 1.4426950408889634f, kSlack = 20.0f;
-  __device__ static __forceinline__ bool plain(float x) { return fabsf(x) < 1e38f; }
-  __device__ __forceinline__ void rescale() {
-    const float by = plain(ref) ? exp2_fast(R - top * kLog2e) : exp_below(ref, top);
-    sum.x *= by;
-    sum.y *= by;
-    ref = top;
-    R = plain(top) ? top * kLog2e : 0.0f;
-  }
+  static constexpr float kLog2e = 1.4426950408889634f, kSlack = 10.0f;
   template <int EV> __device__ __forceinline__ void add(const float (&x)[EV], float most, int j) {
     next = fmaxf(next, fminf(top, most));
     if (most > top) top = most, at = j;
-    if (top > ref + kSlack) rescale();
-    if (plain(ref)) {
-      const float2 l = make_float2(kLog2e, kLog2e), r = make_float2(-R, -R);
+    if (top > ref + kSlack) {
+      const float by = exp2_fast((ref - top) * kLog2e);
+      sum.x *= by;
+      sum.y *= by;
+      ref = top;
+    }
+    const float2 l = make_float2(kLog2e, kLog2e), r = make_float2(-ref, -ref);
 #pragma unroll
-      for (int e = 0; e < EV; e += 2) {
-        float2 t = __ffma2_rn(make_float2(x[e], x[e + 1]), l, r);
-        t.x = exp2_fast(t.x);
-        t.y = exp2_fast(t.y);
-        sum = __fadd2_rn(sum, t);
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < EV; ++e) (e % 2 ? sum.y : sum.x) += exp_below(x[e], ref);
+    for (int e = 0; e < EV; e += 2) {
+      float2 t = __fmul2_rn(__fadd2_rn(make_float2(x[e], x[e + 1]), r), l);
+      t.x = exp2_fast(t.x);
+      t.y = exp2_fast(t.y);
+      sum = __fadd2_rn(sum, t);
     }
   }
-  // sum of exp(x - top)
+  // sum of exp(x - top); the product with log2(e) to twice 32 bits, since ref may be far from top
   __device__ __forceinline__ float relative() const {
-    const float s = sum.x + sum.y;
-    return plain(ref) ? s * exp2f(-fmaf(top, kLog2e, -R)) : top > ref ? s * exp_below(ref, top) : s;
+    const float s = sum.x + sum.y, d = ref - top;
+    if (!(d > -1e30f) || !(d < 1e30f)) return s;   // nothing but -inf, or NaN
+    const float hi = d * kLog2e, lo = fmaf(d, kLog2e, -hi);
+    return s * fmaf(exp2f(hi), lo * 0.6931472f, exp2f(hi));
   }
 };
 

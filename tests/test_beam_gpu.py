@@ -174,6 +174,15 @@ def test_ties_go_to_the_lowest(V, dtype):
     s, p, t = fr.beam_select(rows, torch.zeros(1, 9, device="cuda"), 9)
     assert torch.equal(p[0].cpu(), torch.arange(9)), p
     assert (t == t[0, 0]).all() and (s == s[0, 0]).all()
+    # and rows that differ by a constant
+    whole = torch.randint(-9, 9, (V,), generator=g).to("cuda", TYPES[dtype])
+    rows = whole + torch.tensor([0, 5, -3, 64, 1], dtype=TYPES[dtype], device="cuda")[None, :, None]
+    s, p, t = fr.beam_select(rows, torch.zeros(1, 5, device="cuda"), 5)
+    n = min(5, int((whole == whole.max()).sum()))
+    ties = (whole == whole.max()).nonzero()[:n, 0]
+    assert (p[0, :n] == 0).all() and torch.equal(t[0, :n], ties) and (s[0, :n] == s[0, 0]).all()
+    if n == 1:
+        assert torch.equal(p[0].cpu(), torch.arange(5)) and (s == s[0, 0]).all()
 
 
 @pytest.mark.parametrize("dtype", list(TYPES))
