@@ -132,14 +132,15 @@ template <typename real, int VEC> __device__ __forceinline__ void get(const real
 // counted there by an mbarrier (st.async: a cluster barrier would wait for the stores of h or of
 // the gradients too, a microsecond a turn).  Two buffers in turn are enough: who sends for turn
 // n + 2 has received everybody's composition of turn n + 1, which they sent after they had read
-// turn n's.  Waits are bounded; one that runs out makes the CTA go on with NaN for the state,
-// which reaches all that depends on it.
+// turn n's.  Waits are bounded; one that runs out makes the CTA go on with NaN for the state and
+// send nothing more, so that the waits of the others for it run out in their turn: NaN reaches all
+// that depends on what did not arrive, and no message can be taken for one of another turn.
 constexpr int kRecTries = 1 << 20;
 
 struct RecMail {
   void *slots;       // [2][ranks][kWidth][2]
   uint64_t *bars;    // [2]
-  int rank, ranks;
+  int rank, ranks, tries;
   bool failed;
 };
 __device__ __forceinline__ uint32_t peer_address(const void *p, int rank) {
@@ -177,6 +178,7 @@ template <typename S>
 __device__ __forceinline__ void mail_send(typename S::real A, typename S::real B, int n, const RecMail &mail,
                                           const RecPlace<S> &at) {
   using real = typename S::real;
+  if (mail.failed) return;
   const int buffer = n & 1;
   const real *slots = (const real *)mail.slots + buffer * mail.ranks * 2 * S::kWidth;
   if (threadIdx.x == 0)
@@ -198,7 +200,7 @@ __device__ __forceinline__ typename S::real mail_join(typename S::real &carry, i
   const real *slots = (const real *)mail.slots + buffer * mail.ranks * 2 * S::kWidth;
   const uint32_t bar = (uint32_t)__cvta_generic_to_shared(mail.bars + buffer);
   bool arrived = false;
-  for (int i = 0; !mail.failed && !arrived && i < kRecTries; ++i) {
+  for (int i = 0; !mail.failed && !arrived && i < mail.tries; ++i) {
     uint32_t done;
     asm volatile("{\n.reg .pred q;\nmbarrier.try_wait.parity.shared::cta.b64 q, [%1], %2;\n"
                  "selp.u32 %0, 1, 0, q;\n}"
@@ -227,7 +229,7 @@ __global__ void __launch_bounds__(kRecThreads, 4)
 recurrence_forward_kernel(RecTensor x, RecTensor gate, const typename S::real *__restrict__ initial,
                           const int64_t *__restrict__ lengths, typename S::T *__restrict__ h,
                           typename S::real *__restrict__ last, typename S::real *__restrict__ saved, int steps,
-                          int D) {
+                          int D, int tries) {
   using T = typename S::T;
   using real = typename S::real;
   using Pack = RecPack<T, S::VEC>;
@@ -237,7 +239,7 @@ recurrence_forward_kernel(RecTensor x, RecTensor gate, const typename S::real *_
   real *const exchange = reinterpret_cast<real *>(smem + 4 * S::kStage);   // [2][A, B][kExchange]
   const int rank = CLUSTER ? blockIdx.x : 0, ranks = CLUSTER ? gridDim.x : 1;
   real *const slots = exchange + 4 * S::kExchange;
-  RecMail mail{slots, reinterpret_cast<uint64_t *>(slots + 4 * ranks * S::kWidth), rank, ranks, false};
+  RecMail mail{slots, reinterpret_cast<uint64_t *>(slots + 4 * ranks * S::kWidth), rank, ranks, tries, false};
   const int b = blockIdx.z;
   const RecPlace<S> at(blockIdx.y, D);
   const int n = steps_of(lengths, b, steps), chunks = (steps + kRecChunk - 1) / kRecChunk;
@@ -362,7 +364,7 @@ recurrence_backward_kernel(RecTensor x, RecTensor gate, const int64_t *__restric
                            const typename S::real *__restrict__ saved, RecTensor dh,
                            const typename S::real *__restrict__ dlast, typename S::T *__restrict__ dx,
                            typename S::T *__restrict__ dgate, typename S::real *__restrict__ dinitial, int steps,
-                           int D) {
+                           int D, int tries) {
   using T = typename S::T;
   using real = typename S::real;
   using Pack = RecPack<T, S::VEC>;
@@ -372,7 +374,7 @@ recurrence_backward_kernel(RecTensor x, RecTensor gate, const int64_t *__restric
   real *const exchange = reinterpret_cast<real *>(smem + 6 * S::kStage);   // [2][A, B, M][kExchange]
   const int rank = CLUSTER ? blockIdx.x : 0, ranks = CLUSTER ? gridDim.x : 1;
   real *const slots = exchange + 6 * S::kExchange;
-  RecMail mail{slots, reinterpret_cast<uint64_t *>(slots + 4 * ranks * S::kWidth), rank, ranks, false};
+  RecMail mail{slots, reinterpret_cast<uint64_t *>(slots + 4 * ranks * S::kWidth), rank, ranks, tries, false};
   const int b = blockIdx.z;
   const RecPlace<S> at(blockIdx.y, D);
   const int n = steps_of(lengths, b, steps), chunks = (steps + kRecChunk - 1) / kRecChunk;
@@ -651,19 +653,20 @@ static bool rec_aligned(const RecTensor &t, int size, int D, int bytes) {
 
 template <typename S>
 static int forward_as(const RecTensor &x, const RecTensor &gate, const void *initial, const int64_t *lengths, void *h,
-                      void *last, void *saved, int B, int T, int D, cudaStream_t st) {
+                      void *last, void *saved, int B, int T, int D, int tries, cudaStream_t st) {
   using real = typename S::real;
   return rec_launch<S>(recurrence_forward_kernel<S, false>, recurrence_forward_kernel<S, true>, 2, B, T, D, st, x, gate,
-                       (const real *)initial, lengths, (typename S::T *)h, (real *)last, (real *)saved, T, D);
+                       (const real *)initial, lengths, (typename S::T *)h, (real *)last, (real *)saved, T, D,
+                       tries);
 }
 template <typename S>
 static int backward_as(const RecTensor &x, const RecTensor &gate, const int64_t *lengths, const void *saved,
                        const RecTensor &dh, const void *dlast, void *dx, void *dgate, void *dinitial, int B, int T,
-                       int D, cudaStream_t st) {
+                       int D, int tries, cudaStream_t st) {
   using real = typename S::real;
   return rec_launch<S>(recurrence_backward_kernel<S, false>, recurrence_backward_kernel<S, true>, 3, B, T, D, st, x,
                        gate, lengths, (const real *)saved, dh, (const real *)dlast, (typename S::T *)dx,
-                       (typename S::T *)dgate, (real *)dinitial, T, D);
+                       (typename S::T *)dgate, (real *)dinitial, T, D, tries);
 }
 
 // Vectors of 16 bytes where every row allows them, else of 4 bytes (a float, or a pair of 16-bit
@@ -713,7 +716,7 @@ extern "C" int frnnt_recurrence_forward(int dtype, const void *x, long long x_ba
   };
   const bool wide = fits(16), pairs = fits(4);
 #define FRNNT_REC_FORWARD(...) \
-  forward_as<__VA_ARGS__>(X, G, initial, lengths, h, last, saved, B, T, D, (cudaStream_t)stream)
+  forward_as<__VA_ARGS__>(X, G, initial, lengths, h, last, saved, B, T, D, kRecTries, (cudaStream_t)stream)
   FRNNT_REC_SHAPES(FRNNT_REC_FORWARD, wide, pairs)
 #undef FRNNT_REC_FORWARD
 }
@@ -737,9 +740,22 @@ extern "C" int frnnt_recurrence_backward(int dtype, const void *x, long long x_b
   const bool wide = fits(16), pairs = fits(4);
 #define FRNNT_REC_BACKWARD(...)                                                              \
   backward_as<__VA_ARGS__>(X, G, lengths, saved, DH, dlast, dx, dgate, dinitial, B, T, D,    \
-                           (cudaStream_t)stream)
+                           kRecTries, (cudaStream_t)stream)
   FRNNT_REC_SHAPES(FRNNT_REC_BACKWARD, wide, pairs)
 #undef FRNNT_REC_BACKWARD
+}
+
+extern "C" int frnnt_recurrence_limited(const float *x, const float *gate, float *h, float *last, void *saved,
+                                        const float *dh, float *dx, float *dgate, int B, int T, int D, int tries,
+                                        void *stream) {
+  FRNNT_REQUIRE(B >= 1 && T >= 1 && D >= 1, FRNNT_EINVAL, "bad sizes");
+  FRNNT_REQUIRE(x && gate && h && last && dh && dx && dgate && (saved || T <= kRecChunk), FRNNT_EINVAL, "NULL argument");
+  if (tries < 0) tries = kRecTries;
+  using S = RecShape<float, 1, 16>;
+  const RecTensor X{x, (long long)T * D, D}, G{gate, (long long)T * D, D}, DH{dh, (long long)T * D, D};
+  const int rc = forward_as<S>(X, G, nullptr, nullptr, h, last, saved, B, T, D, tries, (cudaStream_t)stream);
+  if (rc != FRNNT_OK) return rc;
+  return backward_as<S>(X, G, nullptr, saved, DH, nullptr, dx, dgate, nullptr, B, T, D, tries, (cudaStream_t)stream);
 }
 
 extern "C" int frnnt_recurrence_step(int dtype, const void *x, long long x_row, const void *gate,

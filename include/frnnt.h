@@ -28,7 +28,7 @@
  *     the call (nothing synchronises, so the host cannot know): the affected
  *     outputs are poisoned with NaN instead -- ans[b] of the forward recursion,
  *     the first in-box gradient entry (and origin_grad[b]) of the reverse sweep,
- *     the output tile of a tensor-core product.
+ *     the output tile of a tensor-core product, the states of a gated recurrence.
  *
  * Lattice layouts (identical to the reference's tensors):
  *   px   [B][S][T1]     T1 = T+1 ("regular") or T ("modified"/"constrained")
@@ -446,6 +446,15 @@ int frnnt_recurrence_backward(int dtype, const void *x, long long x_batch, long 
                               const void *saved, const void *dh, long long dh_batch, long long dh_step,
                               const void *dlast, void *dx, void *dgate, void *dinitial, int B, int T, int D,
                               void *stream);
+
+/* Forward and backward in float32 (contiguous, no initial state, no lengths) with the waits between
+ * the CTAs of a cluster bounded by so many looks (negative: the usual bound; 0: every wait runs
+ * out at once), to see what a caller gets when one does: NaN in every h, last, dx and dgate that
+ * depends on what did not arrive, and no error, since nothing synchronises.  Sequences of up to
+ * 128 steps, and grids that fill the GPU without clusters, need no waits. */
+int frnnt_recurrence_limited(const float *x, const float *gate, float *h, float *last, void *saved,
+                             const float *dh, float *dx, float *dgate, int B, int T, int D, int tries,
+                             void *stream);
 
 /* One step of `rows` rows of D channels, x and gate with x_row / gate_row elements between rows:
  * row r goes on from state[r], or with parents [rows] from state[(r / beams) * K + parents[r]]

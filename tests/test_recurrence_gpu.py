@@ -294,6 +294,28 @@ def test_offsets_beyond_32_bits():
     check(dx[:, -300:], want["dx"], "dx")
 
 
+@pytest.mark.parametrize("tries", [-1, 0])
+def test_waits_of_a_cluster_that_run_out(tries):
+    """Nothing is withheld: with no looks at all every wait gives up, and the outputs say so."""
+    from fast_rnnt_b200 import _lib
+    B, T, D = 2, 1000, 40
+    x, gate, m = make(B, T, D, torch.float32, seed=21)
+    h, dx, dgate = (torch.empty_like(x) for _ in range(3))
+    last = torch.empty(B, D, device="cuda")
+    saved = torch.empty(_lib.size_of("frnnt_recurrence_saved_bytes", 0, B, T, D), dtype=torch.uint8, device="cuda")
+    _lib.call("frnnt_recurrence_limited", *[_lib.ptr(t) for t in (x, gate, h, last, saved, m["dh"], dx, dgate)],
+              B, T, D, tries, _lib.stream_ptr(x.device))
+    torch.cuda.synchronize()
+    if tries < 0:
+        want = recurrence(x, gate, dh=m["dh"])
+        compare(dict(h=h, last=last, dx=dx, dgate=dgate), want)
+    else:
+        for t in (h, last, dx, dgate):
+            assert torch.isnan(t).all()
+    # and the next call is none the worse for it
+    compare(run(x, gate, dh=m["dh"]), recurrence(x, gate, dh=m["dh"]))
+
+
 # ------------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype", list(TYPES))
 @pytest.mark.parametrize("shape", [(1,), (7,), (5, 64), (3, 4, 37), (1, 1, 1), (2, 3, 4, 8)])
