@@ -471,7 +471,8 @@ int frnnt_recurrence_step(int dtype, const void *x, long long x_row, const void 
 /* The `beam` (1 to 32) best of the K * V continuations of each of B utterances, K at most 1024,
  *   scores[b][i] + logits[b][i][v] - log(sum_v exp(logits[b][i][v])),
  * in out_scores, out_parents (i) and out_tokens (v) [B][beam], best first, compared in 64 bits,
- * equal ones in the order of i * V + v.  dtype (FRNNT_F32, _F16, _BF16) is that of logits, whose rows hold V values
+ * equal ones in the order of i * V + v; a row offers its `beam` largest logits, of equal ones those
+ * of the lowest v.  dtype (FRNNT_F32, _F16, _BF16) is that of logits, whose rows hold V values
  * side by side, `batch` / `row` elements apart.  finished [B][K] (bytes; NULL: none): a set byte
  * leaves the row one continuation, `blank`, at its score.  A score of +-inf or NaN, a logit of
  * -inf and a row without a finite log-sum offer nothing; slots left over hold -inf, -1, -1.
