@@ -23,13 +23,13 @@ def beam_select(logits: Tensor, scores: Tensor, beam: int, termination_symbol: i
         scores[b, i] + log_softmax(logits[b, i])[v]
 
     and where ``finished`` (bool [B][K]) is set it only goes on with termination_symbol, at no
-    cost, its logits not read.  parents and tokens are int64: what continuation [b][j] goes on
+    cost, whatever its logits.  parents and tokens are int64: what continuation [b][j] goes on
     from, and with what.  A hypothesis offers the ``beam`` symbols of its largest logits (of equal
     ones the lowest symbols), and of all offers the best scores win, compared in 64 bits with
     log-sums good to about 1e-7; equal scores go to the lower hypothesis and then to the lower
     symbol.  Equal rows, and rows that differ by a constant, have equal log-softmaxes to the last bit.
 
-    A hypothesis with a score of -inf, +inf or NaN is none (its logits are not read), a symbol whose
+    A hypothesis with a score of -inf, +inf or NaN is none, whatever its logits; a symbol whose
     logit is -inf is never chosen, and a row whose log-sum-exp is not a finite number (a NaN or
     +inf in it, or nothing but -inf) offers nothing.  Where fewer than ``beam`` continuations are
     left, the slots behind them hold a score of -inf and -1 as parent and token, which
