@@ -278,6 +278,18 @@ def test_reorder(B, K, k):
     assert fr.beam_reorder([], parents) == []
 
 
+@pytest.mark.parametrize("dtype", [torch.uint8, torch.bfloat16, torch.float32, torch.int64])
+def test_reorder_rows_of_every_length_and_place(dtype):
+    """Rows that begin anywhere, source and destination each on its own."""
+    import fast_rnnt_b200 as fr
+    g = torch.Generator().manual_seed(9)
+    parents = torch.randint(-1, 5, (3, 4), generator=g).cuda()
+    wide = torch.randint(0, 120, (3, 5, 300), generator=g).to("cuda", dtype)
+    states = [wide[:, :, o:o + n] for n in (1, 2, 3, 7, 15, 16, 17, 31, 33, 63, 64, 65, 79, 97, 255, 280) for o in (0, 1, 5)]
+    for t, u in zip(states, fr.beam_reorder(states, parents)):
+        assert torch.equal(u.cpu(), reordered(t, parents)), t.shape
+
+
 def test_reorder_many_and_large():
     import fast_rnnt_b200 as fr
     g = torch.Generator().manual_seed(7)
