@@ -60,8 +60,12 @@ class GraphedStep:
         # leaves of the capture's own over the same memory: an eager graph of the caller's leaves that
         # is still alive holds their gradient accumulators on its own stream, which a capture
         # cannot wait for
-        own = {k: v.detach().requires_grad_(True) if k in names and v.is_leaf else v
-               for k, v in inputs.items()}
+        made, pairs, own = {}, {}, dict(inputs)
+        for k in names:
+            v = inputs[k]
+            if v.is_leaf:   # one for a tensor that goes by two names
+                own[k] = made.setdefault(id(v), v.detach().requires_grad_(True))
+                pairs[k] = (v, own[k])
         torch.cuda.synchronize(dev)
         torch.cuda.empty_cache()   # the warm-up's scratch, or it stays cached beside the graph's
         n0 = _lib.lib().frnnt_launch_count()
@@ -69,11 +73,10 @@ class GraphedStep:
             self.loss = fn(own)
         self.launches = int(_lib.lib().frnnt_launch_count() - n0)
         for k, v in own.items():
-            if v is not inputs.get(k):
-                if k in inputs:
-                    inputs[k].grad = v.grad
-                else:
-                    inputs[k] = v   # what `fn` put there
+            if k not in pairs or v is not pairs[k][1]:
+                inputs[k] = v      # what `fn` put there
+        for leaf, v in pairs.values():
+            leaf.grad = v.grad
 
     def __call__(self) -> Tensor:
         self.graph.replay()

@@ -103,6 +103,25 @@ def test_pruned_training_step_runs_and_is_captured():
         assert torch.equal(leaves[k].grad, grads[k]), k
 
 
+def test_captured_leaf_with_two_names():
+    import fast_rnnt_b200 as fr
+    from fast_rnnt_b200.graphs import GraphedStep
+    g = torch.Generator().manual_seed(5)
+    x = torch.randn(2, 40, 24, generator=g).cuda().requires_grad_(True)
+
+    def step(t):
+        loss = fr.gated_recurrence(t["x"], t["gate"])[0].square().sum()
+        loss.backward()
+        return loss
+
+    step(dict(x=x, gate=x))
+    want, x.grad = x.grad, None
+    graph = GraphedStep(step, dict(x=x, gate=x))
+    graph()
+    torch.cuda.synchronize()
+    assert torch.equal(x.grad, want)
+
+
 def test_search():
     """A search over the frames: at most one symbol a frame (blank 0 keeps the state), four
     hypotheses.  The formula in 64 bits follows the search's own choices; at every frame the kept
