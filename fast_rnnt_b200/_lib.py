@@ -28,7 +28,7 @@ _ARGUMENTS = {
     "frnnt_recurrence_backward": "ipllpllpppllppppiiip",
     "frnnt_recurrence_step": "iplplppppliiip",
     "frnnt_beam_select": "ipllppippppiiiip",
-    "frnnt_beam_reorder": "ipppppp" + "iiip",
+    "frnnt_beam_reorder": "ippiiip",
 }
 
 

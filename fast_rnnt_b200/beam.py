@@ -8,7 +8,7 @@ import torch
 from torch import Tensor
 
 from . import _lib
-from ._lib import _c_longlong, _c_vp
+from ._lib import _c_longlong
 
 
 def beam_select(logits: Tensor, scores: Tensor, beam: int, termination_symbol: int = 0,
@@ -86,8 +86,8 @@ def beam_reorder(states: Union[Tensor, Sequence[Tensor]], parents: Tensor) -> Un
         return []
     assert tensors[0].ndim >= 2 and tensors[0].shape[1] >= 1, tensors[0].shape
     K, grad = tensors[0].shape[1], torch.is_grad_enabled()
-    start, target, pitch, step, row, out = [], [], [], [], [], []
-    held = []   # copies stay until the launch
+    rows, out = [], []   # rows: from, to, batch and beam strides, bytes of every tensor
+    held = []            # copies stay until the launch
     shape = dtype = None
     with _lib.on_device(dev):
         for t in tensors:
@@ -99,23 +99,16 @@ def beam_reorder(states: Union[Tensor, Sequence[Tensor]], parents: Tensor) -> Un
             assert t.device == dev, (t.device, dev)
             assert not (grad and t.requires_grad), \
                 "beam_reorder has no gradients: call it under torch.no_grad()"
-            if t.is_contiguous():
-                pitch.append(K * bytes_)
-                step.append(bytes_)
-            else:   # a row of a state has to lie in one piece; rows themselves may lie anywhere
+            pitch, step = K * bytes_, bytes_
+            if not t.is_contiguous():   # a row of a state has to lie in one piece; rows may lie anywhere
                 if B > 0 and not t[0, 0].is_contiguous():
                     t = t.contiguous()
-                pitch.append(size * t.stride(0))
-                step.append(size * t.stride(1))
+                pitch, step = size * t.stride(0), size * t.stride(1)
                 held.append(t)
             new = (torch.empty_like(t, memory_format=torch.contiguous_format) if k == K
                    else t.new_empty((B, k) + shape[2:]))
             out.append(new)
-            start.append(t.data_ptr())
-            target.append(new.data_ptr())
-            row.append(bytes_)
-        n = len(out)
-        words, pointers = _c_longlong * n, _c_vp * n
-        _lib.call("frnnt_beam_reorder", n, pointers(*start), words(*pitch), words(*step),
-                  pointers(*target), words(*row), parents.data_ptr(), B, k, K, _lib.stream_ptr(dev))
+            rows += (t.data_ptr(), new.data_ptr(), pitch, step, bytes_)
+        _lib.call("frnnt_beam_reorder", len(out), (_c_longlong * len(rows))(*rows), parents.data_ptr(), B, k, K,
+                  _lib.stream_ptr(dev))
     return out[0] if one else out

@@ -770,16 +770,16 @@ extern "C" int frnnt_beam_select(int dtype, const void *logits, long long batch,
 #undef FRNNT_SELECT
 }
 
-extern "C" int frnnt_beam_reorder(int count, const void *const *from, const long long *batch, const long long *beam,
-                                  void *const *to, const long long *bytes, const int64_t *parents, int B, int beams,
-                                  int K, void *stream) {
+extern "C" int frnnt_beam_reorder(int count, const frnnt_rows *tensors, const int64_t *parents, int B, int beams, int K,
+                                  void *stream) {
   FRNNT_REQUIRE(count >= 0 && B >= 0 && beams >= 0 && K >= 1, FRNNT_EINVAL, "bad sizes");
   const long long rows = (long long)B * beams;
   if (count == 0 || rows == 0) return FRNNT_OK;
-  FRNNT_REQUIRE(from && batch && beam && to && bytes && parents, FRNNT_EINVAL, "NULL argument");
+  FRNNT_REQUIRE(tensors && parents, FRNNT_EINVAL, "NULL argument");
   for (int n = 0; n < count; ++n) {
-    FRNNT_REQUIRE(bytes[n] >= 0 && (bytes[n] == 0 || (from[n] && to[n])), FRNNT_EINVAL, "NULL argument");
-    FRNNT_REQUIRE(bytes[n] == 0 || from[n] != to[n], FRNNT_EINVAL, "a tensor cannot be reordered in place");
+    const frnnt_rows &t = tensors[n];
+    FRNNT_REQUIRE(t.bytes >= 0 && (t.bytes == 0 || (t.from && t.to)), FRNNT_EINVAL, "NULL argument");
+    FRNNT_REQUIRE(t.bytes == 0 || t.from != t.to, FRNNT_EINVAL, "a tensor cannot be reordered in place");
   }
   cudaStream_t st = (cudaStream_t)stream;
   // two kinds of rows: those moved in pieces of their alignment (8 or 16 bytes, or short), and shifted ones
@@ -788,18 +788,19 @@ extern "C" int frnnt_beam_reorder(int count, const void *const *from, const long
     int m = 0;
     long long blocks = 1;
     for (int n = 0; n < count; ++n) {
-      const unsigned long long low = (uintptr_t)from[n] | (uintptr_t)to[n] | (unsigned long long)batch[n] |
-                                     (unsigned long long)beam[n] | (unsigned long long)bytes[n];
+      const frnnt_rows &t = tensors[n];
+      const unsigned long long low = (uintptr_t)t.from | (uintptr_t)t.to | (unsigned long long)t.batch |
+                                     (unsigned long long)t.beam | (unsigned long long)t.bytes;
       const int width = low % 16 == 0 ? 16 : low % 8 == 0 ? 8 : low % 4 == 0 ? 4 : low % 2 == 0 ? 2 : 1;
-      if (bytes[n] > 0 && (width <= 4 && bytes[n] >= 64) == (shifted == 1)) {
-        list.from[m] = (const char *)from[n];
-        list.to[m] = (char *)to[n];
-        list.batch[m] = batch[n];
-        list.beam[m] = beam[n];
-        list.bytes[m] = bytes[n];
+      if (t.bytes > 0 && (width <= 4 && t.bytes >= 64) == (shifted == 1)) {
+        list.from[m] = (const char *)t.from;
+        list.to[m] = (char *)t.to;
+        list.batch[m] = t.batch;
+        list.beam[m] = t.beam;
+        list.bytes[m] = t.bytes;
         list.width[m] = width;
         ++m;
-        const long long pieces = rows * (shifted ? bytes[n] / 16 + 2 : bytes[n] / width);
+        const long long pieces = rows * (shifted ? t.bytes / 16 + 2 : t.bytes / width);
         const long long need = (pieces + kReorderThreads * kReorderPieces - 1) / (kReorderThreads * kReorderPieces);
         blocks = need > blocks ? need : blocks;
       }

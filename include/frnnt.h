@@ -482,13 +482,17 @@ int frnnt_beam_select(int dtype, const void *logits, long long batch, long long 
                       const uint8_t *finished, int blank, float *out_scores, int64_t *out_parents,
                       int64_t *out_tokens, void *scratch, int B, int K, int V, int beam, void *stream);
 
-/* to[n][b][j] = from[n][b][parents[b][j]] for `count` tensors of rows of bytes[n] bytes, zeros
- * where a parent is not in 0 .. K-1.  The five arrays are HOST arrays of `count` entries, read
- * before the call returns; batch and beam are the strides of from[n] in bytes, to[n]
- * [B][beams][bytes[n]] is contiguous and may not overlap from[n]. */
-int frnnt_beam_reorder(int count, const void *const *from, const long long *batch, const long long *beam,
-                       void *const *to, const long long *bytes, const int64_t *parents, int B, int beams,
-                       int K, void *stream);
+/* to[b][j] = from[b][parents[b][j]] for `count` tensors of rows of `bytes` bytes, zeros where a
+ * parent is not in 0 .. K-1.  `rows` is a HOST array of `count` entries, read before the call
+ * returns; batch and beam are the strides of `from` in bytes, `to` [B][beams][bytes] is contiguous
+ * and may not overlap `from`. */
+typedef struct frnnt_rows {
+  const void *from;
+  void *to;
+  long long batch, beam, bytes;
+} frnnt_rows;
+int frnnt_beam_reorder(int count, const frnnt_rows *rows, const int64_t *parents, int B, int beams, int K,
+                       void *stream);
 
 #ifdef __cplusplus
 }

@@ -80,7 +80,7 @@ def test_c_abi_checks(fr):
     refused(*select(0, 1, 1025, 5, 2), code=-2, text=b"beams")
     refused(*select(0, 1, 1000, 1 << 22, 2), code=-2, text=b"2^31")
     refused(*select(0, 1, 2, 5, 2, one, 5), text=b"termination")
-    refused("frnnt_beam_reorder", -1, None, None, None, None, None, one, 1, 1, 1, None, text=b"sizes")
-    p, s = (ctypes.c_void_p * 1)(16), (n * 1)(16)
-    refused("frnnt_beam_reorder", 1, p, s, s, p, s, one, 1, 1, 1, None, text=b"in place")
-    refused("frnnt_beam_reorder", 1, p, s, s, (ctypes.c_void_p * 1)(), s, one, 1, 1, 1, None, text=b"NULL")
+    refused("frnnt_beam_reorder", -1, None, one, 1, 1, 1, None, text=b"sizes")
+    refused("frnnt_beam_reorder", 1, None, one, 1, 1, 1, None, text=b"NULL")
+    for to, text in ((16, b"in place"), (0, b"NULL")):
+        refused("frnnt_beam_reorder", 1, (n * 5)(16, to, 16, 16, 16), one, 1, 1, 1, None, text=text)
