@@ -597,51 +597,78 @@ static int step_as(const void *x, long long x_row, const void *gate, long long g
 
 // ---- host ----------------------------------------------------------------------------
 
-// CTAs of a cluster: tiles of one sequence at once, doubled as long as the whole grid still fits the
-// three CTAs that a multiprocessor holds (a second turn of the grid costs more than the idle
-// multiprocessors: 1 x 8000 x 1024 bf16, 512 of 444 places 25 + 45 us, 256 of them 20 + 27), no
-// more than the sequence has.  One long sequence of few channels gets 16 (1 x 30011 x 512 fp16:
-// 40 us, with 8 CTAs 55, without a cluster 8 CTAs in all).
-static int ranks_for(long long ctas, int T) {
-  int ranks = 1;
-  while (ranks < kRecMostCluster && ctas * ranks * 2 <= 3 * sm_count() && 2 * ranks <= (T + kRecChunk - 1) / kRecChunk)
-    ranks *= 2;
-  return ranks;
+// CTAs of a cluster: tiles of one sequence at once.  The most for which all clusters are on the GPU
+// together, as the runtime counts them (a cluster stays within a GPC, so the multiprocessors' room
+// alone does not say: of 16 CTAs at two a multiprocessor only 14 clusters fit, of 12 CTAs 21), and no
+// more than the sequence has tiles.  A second round of clusters costs more than idle multiprocessors:
+// backward of 1 x 30011 x 512 fp16 58 us with clusters of 12, 76 with 16; 2 x 3000 x 256 fp32 12 us
+// with 8, 20 with 16.  Within one round, more are faster: forward of 8 x 4096 x 512 bf16 34, 33, 28 and
+// 27 us with 1 to 4.  Above the portable eight that holds up to two CTAs a multiprocessor: 1 x 30011
+// x 512 41 us with 16 (256 CTAs), 54 with 8, but 1 x 8000 x 1024 21 us with 12 (384 CTAs), 19 with 8.
+constexpr int kRecRanks[] = {16, 12, 8, 6, 4, 3, 2};
+constexpr int kRecRankKinds = sizeof(kRecRanks) / sizeof(int);
+
+template <typename S> static size_t rec_smem(int arrays, int ranks) {
+  return 2 * (size_t)arrays * (S::kStage + S::kExchange * sizeof(typename S::real)) +
+         (ranks > 1 ? 4 * ranks * S::kWidth * sizeof(typename S::real) + 16 : 0);
 }
 
 template <typename S, typename... Params, typename... Args>
 static int rec_launch(void (*alone)(Params...), void (*cluster)(Params...), int arrays, int B, int T, int D,
                       cudaStream_t st, Args... args) {
-  const int tiles = (D + S::kWidth - 1) / S::kWidth;
+  const int tiles = (D + S::kWidth - 1) / S::kWidth, chunks = (T + kRecChunk - 1) / kRecChunk;
   FRNNT_REQUIRE(B <= 65535 && tiles <= 65535, FRNNT_EUNSUPPORTED, "B or D too large for the grid");
   FRNNT_REQUIRE(T <= INT_MAX - 4 * kRecMostCluster * kRecChunk, FRNNT_EUNSUPPORTED, "T too large");
-  const int ranks = ranks_for((long long)B * tiles, T);
-  const size_t smem = 2 * (size_t)arrays * (S::kStage + S::kExchange * sizeof(typename S::real)) +
-                      (ranks > 1 ? 4 * ranks * S::kWidth * sizeof(typename S::real) + 16 : 0);
-  void (*kernel)(Params...) = ranks > 1 ? cluster : alone;
-  // the attribute belongs to the kernel on a device: asked for once, for the largest cluster
-  static std::atomic<uint64_t> allowed[2];
-  int dev = 0;
-  FRNNT_CUDA(cudaGetDevice(&dev));
-  const uint64_t bit = 1ull << (dev & 63);
-  if (dev > 63 || !(allowed[ranks > 1].load(std::memory_order_relaxed) & bit)) {
-    const size_t most = smem + (ranks > 1 ? 4 * (kRecMostCluster - ranks) * S::kWidth * sizeof(typename S::real) : 0);
-    FRNNT_CUDA(cudaFuncSetAttribute((const void *)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most));
-    if (ranks > 1) FRNNT_CUDA(cudaFuncSetAttribute((const void *)kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-    allowed[ranks > 1].fetch_or(bit, std::memory_order_relaxed);
-  }
   cudaLaunchConfig_t config = {};
-  config.gridDim = dim3((unsigned)ranks, (unsigned)tiles, (unsigned)B);
   config.blockDim = dim3(kRecThreads);
-  config.dynamicSmemBytes = smem;
   config.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = (unsigned)ranks;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   config.attrs = attr;
-  config.numAttrs = ranks > 1 ? 1 : 0;
-  FRNNT_CUDA(FRNNT_KERNEL(cudaLaunchKernelEx(&config, kernel, args...)));
+  // attributes and room belong to the kernel on a device: asked for once
+  static std::atomic<uint64_t> allowed[2];
+  static std::atomic<int> room[64][kRecRankKinds];   // clusters at once, and one
+  int dev = 0;
+  FRNNT_CUDA(cudaGetDevice(&dev));
+  const uint64_t bit = 1ull << (dev & 63);
+  const auto allow = [&](bool clusters) {
+    if (dev <= 63 && allowed[clusters].load(std::memory_order_relaxed) & bit) return FRNNT_OK;
+    const void *kernel = clusters ? (const void *)cluster : (const void *)alone;
+    const size_t most = rec_smem<S>(arrays, clusters ? kRecMostCluster : 1);
+    FRNNT_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most));
+    if (clusters) FRNNT_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    allowed[clusters].fetch_or(bit, std::memory_order_relaxed);
+    return FRNNT_OK;
+  };
+  const auto shape = [&](int ranks) {
+    config.gridDim = dim3((unsigned)ranks, (unsigned)tiles, (unsigned)B);
+    config.dynamicSmemBytes = rec_smem<S>(arrays, ranks);
+    attr[0].val.clusterDim.x = (unsigned)ranks;
+    config.numAttrs = ranks > 1 ? 1 : 0;
+  };
+  const long long clusters = (long long)B * tiles;
+  int ranks = 1;
+  for (int i = 0; i < kRecRankKinds && ranks == 1; ++i) {
+    const int r = kRecRanks[i];
+    if (r > chunks || clusters * r > (r > 8 ? 2 : 4) * sm_count()) continue;   // four at most fit a multiprocessor
+    int fit = dev <= 63 ? room[dev][i].load(std::memory_order_relaxed) - 1 : -1;
+    if (fit < 0) {
+      const int rc = allow(true);
+      if (rc != FRNNT_OK) return rc;
+      shape(r);
+      if (cudaOccupancyMaxActiveClusters(&fit, cluster, &config) != cudaSuccess) {   // no room for one
+        fit = 0;
+        (void)cudaGetLastError();
+      }
+      if (dev <= 63) room[dev][i].store(fit + 1, std::memory_order_relaxed);
+    }
+    if (clusters <= fit) ranks = r;
+  }
+  const int rc = allow(ranks > 1);
+  if (rc != FRNNT_OK) return rc;
+  shape(ranks);
+  FRNNT_CUDA(FRNNT_KERNEL(cudaLaunchKernelEx(&config, ranks > 1 ? cluster : alone, args...)));
   return FRNNT_OK;
 }
 
