@@ -132,17 +132,25 @@ template <typename real, int VEC> __device__ __forceinline__ void get(const real
 // counted there by an mbarrier (st.async: a cluster barrier would wait for the stores of h or of
 // the gradients too, a microsecond a turn).  Two buffers in turn are enough: who sends for turn
 // n + 2 has received everybody's composition of turn n + 1, which they sent after they had read
-// turn n's.  Waits are bounded; one that runs out makes the CTA go on with NaN for the state and
-// send nothing more, so that the waits of the others for it run out in their turn: NaN reaches all
-// that depends on what did not arrive, and no message can be taken for one of another turn.
+// turn n's.  Waits are bounded; where one runs out the state becomes NaN and the CTA, from the next
+// turn on, sends nothing more, so that the waits of the others for it run out in their turn: NaN
+// reaches all that depends on what did not arrive, and no message can be taken for one of another turn.
 constexpr int kRecTries = 1 << 20;
 
 struct RecMail {
   void *slots;       // [2][ranks][kWidth][2]
   uint64_t *bars;    // [2]
+  int *stops;        // [kRecMostCluster] turns that each CTA sent; INT_MAX: all
+  int *gave_up;      // 0, or the turns that this CTA had sent when a wait of its ran out
   int rank, ranks, tries;
-  bool failed;
+  bool failed;       // whether one did before this turn
 };
+constexpr int kRecMailBytes = 2 * 8 + (kRecMostCluster + 4) * 4;   // behind the slots; whole 16 bytes
+__device__ __forceinline__ RecMail mail_at(void *slots, size_t slot_bytes, int rank, int ranks, int tries) {
+  uint64_t *const bars = reinterpret_cast<uint64_t *>((char *)slots + slot_bytes);
+  int *const stops = reinterpret_cast<int *>(bars + 2);
+  return {slots, bars, stops, stops + kRecMostCluster, rank, ranks, tries, false};
+}
 __device__ __forceinline__ uint32_t peer_address(const void *p, int rank) {
   uint32_t a;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
@@ -158,20 +166,58 @@ __device__ __forceinline__ void send_pair(uint32_t to, double a, double b, uint3
                "l"(__double_as_longlong(a)), "l"(__double_as_longlong(b)), "r"(bar)
                : "memory");
 }
+__device__ __forceinline__ bool mail_wait(uint32_t bar, int parity, int tries) {
+  for (int i = 0; i < tries; ++i) {
+    uint32_t done;
+    asm volatile("{\n.reg .pred q;\nmbarrier.try_wait.parity.shared::cta.b64 q, [%1], %2;\n"
+                 "selp.u32 %0, 1, 0, q;\n}"
+                 : "=r"(done)
+                 : "r"(bar), "r"(parity)
+                 : "memory");
+    if (done != 0) return true;
+  }
+  return false;
+}
+__device__ __forceinline__ void mail_expect(uint32_t bar, int bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
 __device__ __forceinline__ void mail_begin(const RecMail &mail) {
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i)
       asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"((uint32_t)__cvta_generic_to_shared(mail.bars + i)) : "memory");
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    *mail.gave_up = 0;
   }
+  if (threadIdx.x < kRecMostCluster) mail.stops[threadIdx.x] = INT_MAX;
   cooperative_groups::this_cluster().sync();   // all have started, and have their mbarriers
 }
-// Nobody leaves before all have received what was sent to them.  A CTA that gave up waiting has not
-// seen its last values arrive: it stays some fifty times as long as they are under way at most.
-__device__ __forceinline__ void mail_end(const RecMail &mail) {
-  const bool failed = __syncthreads_or(mail.failed);
+// A turn begins.  Waits run out between the two barriers of a turn: here all threads see the same.
+__device__ __forceinline__ void mail_turn(RecMail &mail) { mail.failed = *(volatile int *)mail.gave_up != 0; }
+// Nobody leaves before all that was sent to it has arrived.  A CTA that received every turn has seen
+// that.  One that gave up in turn n has everything up to turn n - 1, and nobody sends it turn n + 2
+// (for which he would need its turn n + 1): what turns n and n + 1 lack of a full one, since others had
+// stopped before, is taken from what their mbarriers expect, and then both complete.
+template <typename S> __device__ __forceinline__ void mail_end(const RecMail &mail, int turns) {
+  __syncthreads();
+  const int sent = *(volatile int *)mail.gave_up;
+  if (sent != 0 && threadIdx.x < mail.ranks)
+    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(peer_address(mail.stops + mail.rank, threadIdx.x)), "r"(sent) : "memory");
   cooperative_groups::this_cluster().sync();
-  for (int i = 0; failed && i < 64; ++i) __nanosleep(1000);
+  if (sent == 0 || threadIdx.x != 0) return;
+  constexpr int kEach = 2 * S::kWidth * (int)sizeof(typename S::real);   // from one CTA
+  const int n = sent - 1;
+  int now = 0, after = 0;   // CTAs that sent turns n and n + 1
+  for (int r = 0; r < mail.ranks; ++r) {
+    now += mail.stops[r] > n;
+    after += n + 1 < turns && mail.stops[r] > n + 1;
+  }
+  const uint32_t bar = (uint32_t)__cvta_generic_to_shared(mail.bars + (n & 1)),
+                 next = (uint32_t)__cvta_generic_to_shared(mail.bars + ((n + 1) & 1));
+  if (now < mail.ranks)
+    asm volatile("mbarrier.complete_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"((mail.ranks - now) * kEach) : "memory");
+  mail_expect(next, after * kEach);
+  mail_wait(bar, (n >> 1) & 1, kRecTries);
+  mail_wait(next, ((n + 1) >> 1) & 1, kRecTries);
 }
 // The composition (A, B) of this CTA's tile to all, in the n-th turn.  For joiners.
 template <typename S>
@@ -182,10 +228,7 @@ __device__ __forceinline__ void mail_send(typename S::real A, typename S::real B
   const int buffer = n & 1;
   const real *slots = (const real *)mail.slots + buffer * mail.ranks * 2 * S::kWidth;
   if (threadIdx.x == 0)
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(
-                     (uint32_t)__cvta_generic_to_shared(mail.bars + buffer)),
-                 "r"(mail.ranks * 2 * S::kWidth * (int)sizeof(real))
-                 : "memory");
+    mail_expect((uint32_t)__cvta_generic_to_shared(mail.bars + buffer), mail.ranks * 2 * S::kWidth * (int)sizeof(real));
   for (int r = at.join_q; r < mail.ranks; r += S::kJoin)
     send_pair(peer_address(slots + (mail.rank * S::kWidth + at.join_c) * 2, r), A, B,
               peer_address(mail.bars + buffer, r));
@@ -193,24 +236,15 @@ __device__ __forceinline__ void mail_send(typename S::real A, typename S::real B
 // The state that the tile starts from.  `carry`: the state before the n-th turn, and after it on
 // return.  FORWARD: in the order of the ranks, else against it.  For joiners.
 template <typename S, bool FORWARD>
-__device__ __forceinline__ typename S::real mail_join(typename S::real &carry, int n, RecMail &mail,
+__device__ __forceinline__ typename S::real mail_join(typename S::real &carry, int n, const RecMail &mail,
                                                       const RecPlace<S> &at) {
   using real = typename S::real;
   const int buffer = n & 1;
   const real *slots = (const real *)mail.slots + buffer * mail.ranks * 2 * S::kWidth;
   const uint32_t bar = (uint32_t)__cvta_generic_to_shared(mail.bars + buffer);
-  bool arrived = false;
-  for (int i = 0; !mail.failed && !arrived && i < mail.tries; ++i) {
-    uint32_t done;
-    asm volatile("{\n.reg .pred q;\nmbarrier.try_wait.parity.shared::cta.b64 q, [%1], %2;\n"
-                 "selp.u32 %0, 1, 0, q;\n}"
-                 : "=r"(done)
-                 : "r"(bar), "r"((n >> 1) & 1)
-                 : "memory");
-    arrived = done != 0;
-  }
-  if (!arrived) {
-    mail.failed = true;
+  if (mail.failed) return carry = real(NAN);
+  if (!mail_wait(bar, (n >> 1) & 1, mail.tries)) {
+    *(volatile int *)mail.gave_up = n + 1;
     return carry = real(NAN);
   }
   real before = carry;
@@ -239,7 +273,7 @@ recurrence_forward_kernel(RecTensor x, RecTensor gate, const typename S::real *_
   real *const exchange = reinterpret_cast<real *>(smem + 4 * S::kStage);   // [2][A, B][kExchange]
   const int rank = CLUSTER ? blockIdx.x : 0, ranks = CLUSTER ? gridDim.x : 1;
   real *const slots = exchange + 4 * S::kExchange;
-  RecMail mail{slots, reinterpret_cast<uint64_t *>(slots + 4 * ranks * S::kWidth), rank, ranks, tries, false};
+  RecMail mail = mail_at(slots, 4 * ranks * S::kWidth * sizeof(real), rank, ranks, tries);
   const int b = blockIdx.z;
   const RecPlace<S> at(blockIdx.y, D);
   const int n = steps_of(lengths, b, steps), chunks = (steps + kRecChunk - 1) / kRecChunk;
@@ -264,6 +298,7 @@ recurrence_forward_kernel(RecTensor x, RecTensor gate, const typename S::real *_
   fetch(0);
   if constexpr (CLUSTER) mail_begin(mail);
   for (int turn = 0; turn < turns; ++turn) {
+    if constexpr (CLUSTER) mail_turn(mail);
     fetch(turn + 1);
     copy_wait<1>();
     const int chunk = turn * ranks + rank, first = chunk * kRecChunk + piece_first;
@@ -355,7 +390,7 @@ recurrence_forward_kernel(RecTensor x, RecTensor gate, const typename S::real *_
       *reinterpret_cast<Pack *>(H + t * D) = rec_pack<T, VEC>(zero);
   }
   if (keeper && rank == 0 && at.join_q == 0) last[(size_t)b * D + join_channel] = carry;
-  if constexpr (CLUSTER) mail_end(mail);
+  if constexpr (CLUSTER) mail_end<S>(mail, turns);
 }
 
 template <typename S, bool CLUSTER>
@@ -374,7 +409,7 @@ recurrence_backward_kernel(RecTensor x, RecTensor gate, const int64_t *__restric
   real *const exchange = reinterpret_cast<real *>(smem + 6 * S::kStage);   // [2][A, B, M][kExchange]
   const int rank = CLUSTER ? blockIdx.x : 0, ranks = CLUSTER ? gridDim.x : 1;
   real *const slots = exchange + 6 * S::kExchange;
-  RecMail mail{slots, reinterpret_cast<uint64_t *>(slots + 4 * ranks * S::kWidth), rank, ranks, tries, false};
+  RecMail mail = mail_at(slots, 4 * ranks * S::kWidth * sizeof(real), rank, ranks, tries);
   const int b = blockIdx.z;
   const RecPlace<S> at(blockIdx.y, D);
   const int n = steps_of(lengths, b, steps), chunks = (steps + kRecChunk - 1) / kRecChunk;
@@ -402,6 +437,7 @@ recurrence_backward_kernel(RecTensor x, RecTensor gate, const int64_t *__restric
   fetch(turns - 1);
   if constexpr (CLUSTER) mail_begin(mail);
   for (int turn = turns - 1; turn >= 0; --turn) {
+    if constexpr (CLUSTER) mail_turn(mail);
     if constexpr (!CLUSTER) fetch(turn - 1);
     const int chunk = turn * ranks + rank, first = chunk * kRecChunk + piece_first;
     real start = real(0);   // the state before the tile
@@ -543,7 +579,7 @@ recurrence_backward_kernel(RecTensor x, RecTensor gate, const int64_t *__restric
     }
   }
   if (dinitial != nullptr && keeper && rank == 0 && at.join_q == 0) dinitial[(size_t)b * D + join_channel] = carry;
-  if constexpr (CLUSTER) mail_end(mail);
+  if constexpr (CLUSTER) mail_end<S>(mail, turns);
 }
 
 // One token: every row reads the state of its parent (its own without parents; zero where the
@@ -610,7 +646,7 @@ constexpr int kRecRankKinds = sizeof(kRecRanks) / sizeof(int);
 
 template <typename S> static size_t rec_smem(int arrays, int ranks) {
   return 2 * (size_t)arrays * (S::kStage + S::kExchange * sizeof(typename S::real)) +
-         (ranks > 1 ? 4 * ranks * S::kWidth * sizeof(typename S::real) + 16 : 0);
+         (ranks > 1 ? 4 * ranks * S::kWidth * sizeof(typename S::real) + kRecMailBytes : 0);
 }
 
 template <typename S, typename... Params, typename... Args>

@@ -363,3 +363,30 @@ def test_steps_are_the_sequence():
     want = recurrence(x, gate, m["initial"])
     check(torch.stack(hs, 1), want["h"], "h")
     check(state, want["last"], "last")
+
+
+@pytest.mark.parametrize("B,T,D", [(2, 1000, 40), (1, 5000, 33), (3, 400, 300), (1, 30011, 64)])
+def test_waits_that_run_out_now_and_then(B, T, D):
+    """However few looks a wait is given: every value is that of waits without a limit, or NaN."""
+    from fast_rnnt_b200 import _lib
+    x, gate, m = make(B, T, D, torch.float32, seed=22)
+
+    def limited(tries):
+        out = dict(h=torch.empty_like(x), last=torch.empty(B, D, device="cuda"), dx=torch.empty_like(x),
+                   dgate=torch.empty_like(x))
+        saved = torch.empty(_lib.size_of("frnnt_recurrence_saved_bytes", 0, B, T, D), dtype=torch.uint8, device="cuda")
+        _lib.call("frnnt_recurrence_limited", *[_lib.ptr(t) for t in (x, gate, out["h"], out["last"], saved, m["dh"],
+                                                                      out["dx"], out["dgate"])],
+                  B, T, D, tries, _lib.stream_ptr(x.device))
+        torch.cuda.synchronize()
+        return out
+
+    want = limited(-1)
+    assert all(torch.isfinite(t).all() for t in want.values())
+    for tries in (0, 1, 2, 3, 5, 9, 20, 50, 0, -1):
+        got = limited(tries)
+        for name, t in got.items():
+            lost = torch.isnan(t)
+            assert torch.equal(torch.where(lost, want[name], t), want[name]), (tries, name)
+        if tries < 0:
+            assert not any(torch.isnan(t).any() for t in got.values())
