@@ -9,6 +9,7 @@ import functools
 import os
 
 import torch
+from torch.autograd import forward_ad
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libfrnnt_sm100.so")
@@ -90,6 +91,13 @@ def ptr(t):
 def stream_ptr(device):
     """The current stream of the device, as the raw pointer torch keeps (no Stream object)."""
     return _c_vp(torch._C._cuda_getCurrentRawStream(device.index))
+
+
+def has_tangent(*tensors) -> bool:
+    """Whether one of the tensors (None: no tensor) carries a tangent of forward-mode
+    differentiation, which no kernel here would carry on."""
+    return forward_ad._current_level >= 0 and any(
+        t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 class _AlreadyCurrent:

@@ -53,6 +53,7 @@ def beam_select(logits: Tensor, scores: Tensor, beam: int, termination_symbol: i
         finished = finished.contiguous()
     assert not (torch.is_grad_enabled() and (logits.requires_grad or scores.requires_grad)), \
         "beam_select has no gradients: call it under torch.no_grad()"
+    assert not _lib.has_tangent(logits, scores), "beam_select has no forward-mode derivative"
     if V > 1 and logits.stride(2) != 1:
         logits = logits.contiguous()
     scores = scores.contiguous()
@@ -99,6 +100,7 @@ def beam_reorder(states: Union[Tensor, Sequence[Tensor]], parents: Tensor) -> Un
             assert t.device == dev, (t.device, dev)
             assert not (grad and t.requires_grad), \
                 "beam_reorder has no gradients: call it under torch.no_grad()"
+            assert not _lib.has_tangent(t), "beam_reorder has no forward-mode derivative"
             pitch, step = K * bytes_, bytes_
             if not t.is_contiguous():   # a row of a state has to lie in one piece; rows may lie anywhere
                 if B > 0 and not t[0, 0].is_contiguous():

@@ -107,7 +107,7 @@ def gated_recurrence(x: Tensor, gate: Tensor, initial: Optional[Tensor] = None,
     A gate of -inf drops the state (h[:, t] = x[:, t]) and one of +inf keeps it.
 
     B is at most 65535.  A sequence has the same bits in any batch.  Differentiable once with
-    respect to x, gate and initial.  No counterpart in the reference."""
+    respect to x, gate and initial, in reverse mode (tensors with a forward-mode tangent are refused).  No counterpart in the reference."""
     assert x.ndim == 3, x.ndim
     shape, dtype, dev = x.shape, x.dtype, x.device
     assert gate.shape == shape, (gate.shape, shape)
@@ -125,8 +125,9 @@ def gated_recurrence(x: Tensor, gate: Tensor, initial: Optional[Tensor] = None,
         assert lengths.device == dev, (lengths.device, dev)
         lengths = lengths.contiguous()
     x, gate = _rows(x), _rows(gate)
-    if torch.is_grad_enabled() and (x.requires_grad or gate.requires_grad or
-                                    (initial is not None and initial.requires_grad)):
+    if (torch.is_grad_enabled() and (x.requires_grad or gate.requires_grad or
+                                     (initial is not None and initial.requires_grad))
+            or _lib.has_tangent(x, gate, initial)):   # the autograd function refuses tangents
         return _GatedRecurrence.apply(x, gate, initial, lengths)
     return _forward(x, gate, initial, lengths, False)[:2]
 
@@ -164,6 +165,7 @@ def gated_recurrence_step(x: Tensor, gate: Tensor, state: Tensor,
     assert not (torch.is_grad_enabled() and (x.requires_grad or gate.requires_grad or
                                              state.requires_grad)), \
         "gated_recurrence_step has no gradients: use gated_recurrence, or torch.no_grad()"
+    assert not _lib.has_tangent(x, gate, state), "gated_recurrence_step has no forward-mode derivative"
     # rows at one distance from the next
     x2 = x if x.is_contiguous() else _rows(x.reshape(-1, D))
     gate2 = gate if gate.is_contiguous() else _rows(gate.reshape(-1, D))
