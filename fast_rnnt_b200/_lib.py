@@ -88,6 +88,12 @@ def ptr(t):
     return _c_vp(t.data_ptr())
 
 
+def plain(t):
+    """`t`, or what it stands for where its memory holds the negative of that (the imaginary part of
+    a lazily conjugated tensor)."""
+    return t.resolve_neg() if t.is_neg() else t
+
+
 def stream_ptr(device):
     """The current stream of the device, as the raw pointer torch keeps (no Stream object)."""
     return _c_vp(torch._C._cuda_getCurrentRawStream(device.index))

@@ -54,9 +54,10 @@ def beam_select(logits: Tensor, scores: Tensor, beam: int, termination_symbol: i
     assert not (torch.is_grad_enabled() and (logits.requires_grad or scores.requires_grad)), \
         "beam_select has no gradients: call it under torch.no_grad()"
     assert not _lib.has_tangent(logits, scores), "beam_select has no forward-mode derivative"
+    logits = _lib.plain(logits)
     if V > 1 and logits.stride(2) != 1:
         logits = logits.contiguous()
-    scores = scores.contiguous()
+    scores = _lib.plain(scores).contiguous()
     code, (sb, sk, _) = _lib.input_code(logits.dtype), logits.stride()
     with _lib.on_device(dev):
         best = torch.empty_like(scores) if beam == K else scores.new_empty((B, beam))
@@ -95,12 +96,15 @@ def beam_reorder(states: Union[Tensor, Sequence[Tensor]], parents: Tensor) -> Un
             if t.shape != shape or t.dtype != dtype:   # tensors of one kind come in rows
                 shape, dtype = t.shape, t.dtype
                 assert len(shape) >= 2 and shape[0] == B and shape[1] == K, (shape, parents.shape, K)
-                size = t.element_size()
+                size, complex_ = t.element_size(), t.is_complex()
                 bytes_ = size * math.prod(shape[2:])
             assert t.device == dev, (t.device, dev)
             assert not (grad and t.requires_grad), \
                 "beam_reorder has no gradients: call it under torch.no_grad()"
             assert not _lib.has_tangent(t), "beam_reorder has no forward-mode derivative"
+            if t.is_neg() or (complex_ and t.is_conj()):   # memory that holds something else
+                t = t.resolve_conj().resolve_neg()
+                held.append(t)
             pitch, step = K * bytes_, bytes_
             if not t.is_contiguous():   # a row of a state has to lie in one piece; rows may lie anywhere
                 if B > 0 and not t[0, 0].is_contiguous():

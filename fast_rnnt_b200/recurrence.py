@@ -27,6 +27,7 @@ def _state_type(dtype):
 
 def _rows(t: Tensor) -> Tensor:
     """`t`, or a copy where its channels do not lie side by side."""
+    t = _lib.plain(t)
     return t if t.shape[-1] <= 1 or t.stride(-1) == 1 else t.contiguous()
 
 
@@ -56,7 +57,7 @@ def _backward(ctx, dh, dlast):
     if dh is not None:
         dh = _rows(dh)
     if dlast is not None:
-        dlast = dlast.contiguous()
+        dlast = _lib.plain(dlast).contiguous()
     with _lib.on_device(dev):
         dx = torch.empty_like(x, memory_format=torch.contiguous_format)
         dgate = torch.empty_like(dx)
@@ -119,7 +120,7 @@ def gated_recurrence(x: Tensor, gate: Tensor, initial: Optional[Tensor] = None,
         assert initial.shape == (shape[0], shape[2]), (initial.shape, shape)
         assert initial.device == dev, (initial.device, dev)
         assert initial.dtype in (state, dtype), initial.dtype
-        initial = (initial if initial.dtype == state else initial.to(state)).contiguous()
+        initial = _lib.plain(initial if initial.dtype == state else initial.to(state)).contiguous()
     if lengths is not None:
         assert lengths.shape == shape[:1] and lengths.dtype == torch.int64, (lengths.shape, lengths.dtype)
         assert lengths.device == dev, (lengths.device, dev)
@@ -166,10 +167,11 @@ def gated_recurrence_step(x: Tensor, gate: Tensor, state: Tensor,
                                              state.requires_grad)), \
         "gated_recurrence_step has no gradients: use gated_recurrence, or torch.no_grad()"
     assert not _lib.has_tangent(x, gate, state), "gated_recurrence_step has no forward-mode derivative"
+    x, gate = _lib.plain(x), _lib.plain(gate)
     # rows at one distance from the next
     x2 = x if x.is_contiguous() else _rows(x.reshape(-1, D))
     gate2 = gate if gate.is_contiguous() else _rows(gate.reshape(-1, D))
-    state = state.contiguous()
+    state = _lib.plain(state).contiguous()
     rows = x.numel() // D if D > 0 else 0
     with _lib.on_device(dev):
         new = torch.empty_like(x, dtype=kind, memory_format=torch.contiguous_format)

@@ -333,3 +333,42 @@ def test_captured_search_step():
         torch.cuda.synchronize()
         for a, b in zip(out, step(*inputs(seed))):
             assert torch.equal(a, b)
+
+
+def test_reorder_of_lazily_conjugated_and_negated_states():
+    """Tensors whose memory holds the conjugate, or the negative, of what they are."""
+    import fast_rnnt_b200 as fr
+    g = torch.Generator().manual_seed(11)
+    z = torch.complex(torch.randn(3, 4, 6, generator=g), torch.randn(3, 4, 6, generator=g)).cuda()
+    parents = torch.randint(-1, 4, (3, 4), generator=g).cuda()
+    states = [z, z.conj(), z.conj()[:, :, 1:], z.conj().imag, z.conj().imag[..., 0], z.conj().real,
+              torch._neg_view(z.real.contiguous())]
+    assert [t.is_conj() or t.is_neg() for t in states] == [False, True, True, True, True, False, True]
+    for t, u in zip(states, fr.beam_reorder(states, parents)):
+        assert torch.equal(u.cpu(), reordered(t.resolve_conj().resolve_neg(), parents))
+
+
+def test_other_inputs_that_are_lazily_negated():
+    """A single channel or symbol, whose memory no copy would set right on the way."""
+    import fast_rnnt_b200 as fr
+    g = torch.Generator().manual_seed(12)
+    for width in (1, 8):
+        z, gate = (torch.complex(*torch.randn(2, 2, 5, width, generator=g)).cuda() for _ in range(2))
+        x, f = z.conj().imag, torch._neg_view(gate.real.contiguous())
+        lazy = [x, f, x[:, 0], f[:, 0]]
+        assert all(t.is_neg() for t in lazy)
+        plain = [t.resolve_neg().contiguous() for t in lazy]
+        for a, b in zip(fr.gated_recurrence(*lazy[:3]), fr.gated_recurrence(*plain[:3])):
+            assert torch.equal(a, b)
+        for a, b in zip(fr.gated_recurrence_step(lazy[2], lazy[3], torch._neg_view(plain[3])),
+                        fr.gated_recurrence_step(plain[2], plain[3], -plain[3])):
+            assert torch.equal(a, b)
+        leaves = [t.clone().requires_grad_(True) for t in plain[:2]]
+        out = fr.gated_recurrence(*leaves)
+        d = [torch._neg_view(t.detach().clone()) for t in out]
+        for a, b in zip(torch.autograd.grad(out, leaves, d, retain_graph=True),
+                        torch.autograd.grad(out, leaves, [t.resolve_neg() for t in d])):
+            assert torch.equal(a, b)
+        for a, b in zip(fr.beam_select(x, torch._neg_view(plain[1][..., 0].contiguous()), 4),
+                        fr.beam_select(plain[0], -plain[1][..., 0], 4)):
+            assert torch.equal(a, b)
