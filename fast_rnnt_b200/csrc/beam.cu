@@ -162,8 +162,9 @@ template <typename T> __device__ __forceinline__ uint4 load_any(const SelRow<T> 
 
 // What a thread keeps of its share of a row.  The sum of exponentials is relative to `ref`, which
 // follows the maximum only when that is far above it: nearly every vector raises some lane's
-// maximum, hardly one needs the sum rescaled.  All of it is arithmetic on differences of logits:
-// rows that differ by a constant (which the subtraction leaves exact) have equal sums.
+// maximum, hardly one needs the sum rescaled.  All of it is arithmetic on differences of logits, and
+// so is what it is decided by: rows that differ by a constant (which the subtraction leaves exact)
+// have equal sums.
 struct SelShare {
   float top = neg_inf<float>(), next = neg_inf<float>(), ref = -FLT_MAX;
   float2 sum = {0, 0};
@@ -172,7 +173,7 @@ struct SelShare {
   template <int EV> __device__ __forceinline__ void add(const float (&x)[EV], float most, int j) {
     next = fmaxf(next, fminf(top, most));
     if (most > top) top = most, at = j;
-    if (top > ref + kSlack) {
+    if (top - ref > kSlack) {
       const float by = exp2_fast((ref - top) * kLog2e);
       sum.x *= by;
       sum.y *= by;

@@ -372,3 +372,28 @@ def test_other_inputs_that_are_lazily_negated():
         for a, b in zip(fr.beam_select(x, torch._neg_view(plain[1][..., 0].contiguous()), 4),
                         fr.beam_select(plain[0], -plain[1][..., 0], 4)):
             assert torch.equal(a, b)
+
+
+def test_rows_that_differ_by_a_constant_rescale_alike():
+    """Logits whose distance is within a rounding of where a thread's sum of exponentials is rescaled:
+    whether it is may not hang on where the row lies."""
+    import fast_rnnt_b200 as fr
+    u = 2.0 ** -20
+    V = 4 * (1 + 128 * 4 + 2)
+    g = torch.Generator().manual_seed(13)
+    # multiples of 2^-20 that a shift by 8 leaves exact
+    base = (torch.randn(V, generator=g, dtype=torch.float64).clamp(-4, 0.5) / u).round() * u - 1
+    rows = []
+    for low, high in ((1.5, 2), (0.5, 1), (2.5, 3), (1.5, 1), (3.5, 3)):
+        row = base.clone()
+        for thread in range(0, 128, 3):
+            row[4 + 4 * thread] = low * u                     # first vector of the thread
+            row[4 + 4 * (thread + 128 * 2)] = 10 + high * u   # a later one, in the same thread's share
+        rows.append(row)
+    for row in rows:
+        for order in ((0.0, -8.0), (-8.0, 0.0)):
+            logits = torch.stack([row + s for s in order]).float()
+            assert torch.equal(logits.double(), torch.stack([row + s for s in order]))
+            _, parents, tokens = fr.beam_select(logits[None].cuda(), torch.zeros(1, 2, device="cuda"), 6)
+            assert not parents.any(), parents
+            assert torch.equal(tokens[0].cpu(), torch.sort(logits[0], descending=True, stable=True).indices[:6])
