@@ -390,3 +390,24 @@ def test_waits_that_run_out_now_and_then(B, T, D):
             assert torch.equal(torch.where(lost, want[name], t), want[name]), (tries, name)
         if tries < 0:
             assert not any(torch.isnan(t).any() for t in got.values())
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_gates_of_long_memory(dtype):
+    """What a step keeps of the state, off by one rounding below 1 (2^-25) and by what the other share
+    is off by: its exponential (2 units in the last place; for 16-bit types those of ex2, the rounding
+    of its argument and that of log2(e), 1.3 |g| units of 2^-24), a sum (half a unit) and a
+    reciprocal (one)."""
+    import fast_rnnt_b200 as fr
+    gate = torch.linspace(0, 17, 40001).to("cuda", TYPES[dtype])[None]
+    zero, one = torch.zeros_like(gate), torch.ones(gate.shape, device="cuda")
+    g = gate.cpu().double()
+    take = torch.sigmoid(-g)
+    bound = 2.0 ** -25 + take * (7 + (0 if dtype == "f32" else 1.3 * g)) * 2.0 ** -24
+    for sign in (1, -1):
+        # a step that keeps the state, and one that takes the input
+        x, state = (zero, one) if sign == 1 else (zero + 1, 0 * one)
+        off = fr.gated_recurrence_step(x, sign * gate, state)[1].cpu().double() - torch.sigmoid(g)
+        assert (off.abs() <= bound).all(), (sign, float((off.abs() / bound).max()))
+        off = fr.gated_recurrence(x[:, None], sign * gate[:, None], state)[1].cpu().double() - torch.sigmoid(g)
+        assert (off.abs() <= bound).all(), (sign, float((off.abs() / bound).max()))
