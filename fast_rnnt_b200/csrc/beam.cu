@@ -498,8 +498,8 @@ select_join_kernel(const SelSum *__restrict__ sums, const uint64_t *__restrict__
       for (int p = 0; p < parts; ++p)
         total += sum[i * parts + p].sum * (double)exp_below(sum[i * parts + p].top, top);
       log_sum = log_of(total);
-      if (fabsf(top) < INFINITY && total < (double)INFINITY)   // no NaN either
-        shift = (float)((double)score - (double)top - log_sum);
+      if (fabsf(top) < INFINITY && total < (double)INFINITY)   // no NaN either; the row offers something
+        shift = fmaxf((float)((double)score - (double)top - log_sum), -FLT_MAX);
     }
     row_log[i] = log_sum;
     row_top[i] = top;

@@ -397,3 +397,16 @@ def test_rows_that_differ_by_a_constant_rescale_alike():
             _, parents, tokens = fr.beam_select(logits[None].cuda(), torch.zeros(1, 2, device="cuda"), 6)
             assert not parents.any(), parents
             assert torch.equal(tokens[0].cpu(), torch.sort(logits[0], descending=True, stable=True).indices[:6])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_scores_and_logits_at_the_ends_of_the_range(dtype):
+    """A score less its row's largest logit may leave 32 bits; the continuation's own score does not."""
+    for top, low in ((1e38, -1e38), (-2e38, -3e38), (1e38, 0.0)):
+        logits = torch.full((1, 3, 500), low, dtype=torch.float64)
+        for i in range(3):
+            logits[0, i, [7 * i + 3, 100 + i]] = top
+        logits = logits.to("cuda", TYPES[dtype])
+        for scores in ([-3e38, -2.9e38, -math.inf], [-3.4e38, -3.4e38, -3.3e38], [0.0, -1e38, -2e38]):
+            scores = torch.tensor([scores], device="cuda")
+            verify(logits, scores, 2 * int((scores > -INF).sum()))
