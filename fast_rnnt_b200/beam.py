@@ -25,9 +25,14 @@ def beam_select(logits: Tensor, scores: Tensor, beam: int, termination_symbol: i
     and where ``finished`` (bool [B][K]) is set it only goes on with termination_symbol, at no
     cost, whatever its logits.  parents and tokens are int64: what continuation [b][j] goes on
     from, and with what.  A hypothesis offers the ``beam`` symbols of its largest logits (of equal
-    ones the lowest symbols), and of all offers the best scores win, compared in 64 bits with
-    log-sums good to about 1e-7; equal scores go to the lower hypothesis and then to the lower
-    symbol.  Equal rows, and rows that differ by a constant, have equal log-softmaxes to the last bit.
+    ones the lowest symbols), and of all offers the best scores win, compared in 64 bits; equal
+    scores go to the lower hypothesis and then to the lower symbol.  The log-sums come from
+    exponentials and sums in 32 bits, off by no more than 2^-21 + (V / 256 + 16) 2^-24 (1.6e-6 for
+    500 symbols, 1.3e-5 for 50 000; measured 3e-7 and 1.2e-6).  Equal rows, and rows that differ by
+    a constant, have equal log-softmaxes to the last bit.
+
+    Two hypotheses with the same symbols and another place of their blanks are two: nothing here
+    merges them.
 
     A hypothesis with a score of -inf, +inf or NaN is none, whatever its logits; a symbol whose
     logit is -inf is never chosen, and a row whose log-sum-exp is not a finite number (a NaN or

@@ -8,7 +8,7 @@
 // the recurrence itself and all that is rounded to the output's type.  Where there are fewer
 // channels than would fill the GPU, a cluster of CTAs takes that many tiles of one sequence at
 // once and joins their compositions through distributed shared memory; the order of all sums
-// depends on the sizes alone.
+// depends on the type, the length and the alignment of the tensors, not on the batch or the cluster.
 //
 // backward: lam_t = dh_t + f_{t+1} lam_{t+1} is the same recurrence from the other end, with the
 // same products of gates.  h_{t-1} is recomputed from the state that the forward keeps per tile:

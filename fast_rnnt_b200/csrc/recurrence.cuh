@@ -124,9 +124,10 @@ template <typename real, int VEC> __device__ __forceinline__ void vset(real (&ou
 // smaller of the two is a product, never the difference of two numbers near one, and the larger is
 // one less that product, rounded once: off by 2^-25 where the other is small.  (As the reciprocal of
 // the rounded 1 + e it was off by up to 2^-23: the state after 30000 steps at a gate of 12 by 1.7e-3,
-// now 1.2e-4; the one instruction more costs a hundredth of the time.)  The reciprocal of 1 .. 2 is the hardware's (within one unit in the
-// last place); for 16-bit inputs the exponential is, too: a relative error of (4 + 1.3 |g|) 2^-24,
-// 2^-17 at most where it is not zero, below the 2^-9 / 2^-12 of their outputs.
+// now 1.2e-4; the one instruction more costs a hundredth of the time.)  The reciprocal of 1 .. 2 is
+// the hardware's (within one unit in the last place); for 16-bit inputs the exponential is, too: a
+// relative error of (4 + 1.3 |g|) 2^-24, 2^-17 at most where it is not zero, below the 2^-9 / 2^-12
+// of their outputs.
 template <typename T> __device__ __forceinline__ RecState<T> rec_exp(RecState<T> x) { return exp_r(x); }
 __device__ __forceinline__ float rec_exp_fast(float x) {
   float y;

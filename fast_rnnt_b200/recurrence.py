@@ -105,9 +105,11 @@ def gated_recurrence(x: Tensor, gate: Tensor, initial: Optional[Tensor] = None,
     Steps t >= lengths[b] of a padded batch are not read and leave the state alone: h is zero
     there and so are the gradients of x and gate; last[b] is the state after lengths[b] steps,
     which is initial[b] for an empty sequence.  Lengths below 0 or above T count as 0 and T.
-    A gate of -inf drops the state (h[:, t] = x[:, t]) and one of +inf keeps it.
+    A gate of -inf drops the state (h[:, t] = x[:, t]) and one of +inf keeps it.  x and the states
+    are finite numbers: behind an infinite one, its channel holds infinities or NaN.
 
-    B is at most 65535.  A sequence has the same bits in any batch.  Differentiable once with
+    B is at most 65535.  A sequence has the same bits in any batch whose tensors are aligned alike
+    (rows on 16 bytes, on 4, or on neither).  Differentiable once with
     respect to x, gate and initial, in reverse mode (tensors with a forward-mode tangent are refused).  No counterpart in the reference."""
     assert x.ndim == 3, x.ndim
     shape, dtype, dev = x.shape, x.dtype, x.device
@@ -142,7 +144,8 @@ def gated_recurrence_step(x: Tensor, gate: Tensor, state: Tensor,
     With ``parents`` (int64 [B][k], as beam_select returns them) x and gate are [B][k][D], state
     is [B][K][D] and row [b][j] goes on from state[b][parents[b][j]]: the reordering of the
     states costs no pass of its own.  A parent outside 0 .. K-1 (-1: no hypothesis) counts as a
-    state of zeros.  state is float32 (float64 for float64 inputs) and is left as it is.
+    state of zeros.  A row whose gate is +inf everywhere keeps its parent's state, bit for bit, and
+    h is that state in the type of x: what a transducer's blank leaves behind.  state is float32 (float64 for float64 inputs) and is left as it is.
 
     Not differentiable: gated_recurrence is for training.  No counterpart in the reference."""
     assert x.ndim >= 1 and gate.shape == x.shape, (gate.shape, x.shape)

@@ -187,3 +187,35 @@ def test_search():
     assert (path[2, :, int(b["frames"][2]):] == 0).all()       # nothing after an utterance's end
     # the hypotheses of an utterance are different paths
     assert all(len({tuple(h.tolist()) for h in path[i]}) == K for i in range(B))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_search_whose_step_keeps_the_state_on_blank(dtype):
+    """A gate of +inf where a hypothesis goes on with blank: its state and output, read through the
+    parents, stay as they are, bit for bit as if they were reordered and selected."""
+    import fast_rnnt_b200 as fr
+    K = 4
+    g = torch.Generator().manual_seed(7)
+    embed, w = (torch.randn(*s, generator=g).cuda().to(dtype) for s in ((C, D), (2 * D, D)))
+    out = torch.randn(C, D, generator=g).cuda()
+    out[0] *= 4      # blank often enough
+    with torch.no_grad():
+        network = lambda tokens: (embed[tokens.clamp(min=0)] @ w.T).chunk(2, -1)   # noqa: E731
+        zero = torch.zeros(B, K, D, device="cuda")
+        dec, state = fr.gated_recurrence_step(*network(torch.zeros(B, K, dtype=torch.int64, device="cuda")), zero)
+        ref_dec, ref_state = dec, state
+        scores = torch.full((B, K), -math.inf, device="cuda")
+        scores[:, 0] = 0
+        seen = set()
+        for t in range(12):
+            frame = torch.randn(B, 1, D, generator=g).cuda()
+            scores, parents, tokens = fr.beam_select(torch.tanh(frame + dec) @ out.T, scores, K)
+            x, gate = network(tokens)
+            emitted = (tokens > 0)[..., None]
+            dec, state = fr.gated_recurrence_step(x, gate.masked_fill(~emitted, math.inf), state, parents)
+            old_dec, old_state = fr.beam_reorder([ref_dec, ref_state], parents)
+            new_dec, new_state = fr.gated_recurrence_step(x, gate, old_state)
+            ref_dec, ref_state = (torch.where(emitted, n, o) for n, o in ((new_dec, old_dec), (new_state, old_state)))
+            assert torch.equal(dec, ref_dec) and torch.equal(state, ref_state), t
+            seen |= set((tokens > 0).flatten().tolist()) | ({None} if (parents < 0).any() else set())
+        assert {True, False} <= seen
