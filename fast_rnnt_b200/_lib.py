@@ -94,16 +94,23 @@ def plain(t):
     return t.resolve_neg() if t.is_neg() else t
 
 
+raw_stream = torch._C._cuda_getCurrentRawStream   # of a device's index, for calls whose arguments have types
+
+
 def stream_ptr(device):
     """The current stream of the device, as the raw pointer torch keeps (no Stream object)."""
     return _c_vp(torch._C._cuda_getCurrentRawStream(device.index))
 
 
+def tangents_possible() -> bool:
+    """Whether forward-mode differentiation is under way."""
+    return forward_ad._current_level >= 0
+
+
 def has_tangent(*tensors) -> bool:
     """Whether one of the tensors (None: no tensor) carries a tangent of forward-mode
     differentiation, which no kernel here would carry on."""
-    return forward_ad._current_level >= 0 and any(
-        t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+    return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 class _AlreadyCurrent:

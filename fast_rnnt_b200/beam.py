@@ -50,7 +50,7 @@ def beam_select(logits: Tensor, scores: Tensor, beam: int, termination_symbol: i
         raise TypeError(f"only float32, float16 and bfloat16 logits are supported, got {logits.dtype}")
     assert scores.dtype == torch.float32, scores.dtype
     dev = logits.device
-    assert logits.is_cuda and scores.device == dev, (dev, scores.device)
+    assert logits.is_cuda and scores.get_device() == dev.index, (dev, scores.device)
     if finished is not None:
         assert finished.shape == (B, K) and finished.dtype == torch.bool, (finished.shape, finished.dtype)
         assert finished.device == dev, (dev, finished.device)
@@ -58,11 +58,12 @@ def beam_select(logits: Tensor, scores: Tensor, beam: int, termination_symbol: i
         finished = finished.contiguous()
     assert not (torch.is_grad_enabled() and (logits.requires_grad or scores.requires_grad)), \
         "beam_select has no gradients: call it under torch.no_grad()"
-    assert not _lib.has_tangent(logits, scores), "beam_select has no forward-mode derivative"
-    logits = _lib.plain(logits)
+    assert not (_lib.tangents_possible() and _lib.has_tangent(logits, scores)), "beam_select has no forward-mode derivative"
+    if logits.is_neg() or scores.is_neg():
+        logits, scores = logits.resolve_neg(), scores.resolve_neg()
     if V > 1 and logits.stride(2) != 1:
         logits = logits.contiguous()
-    scores = _lib.plain(scores).contiguous()
+    scores = scores.contiguous()
     code, (sb, sk, _) = _lib.input_code(logits.dtype), logits.stride()
     with _lib.on_device(dev):
         best = torch.empty_like(scores) if beam == K else scores.new_empty((B, beam))
@@ -73,7 +74,7 @@ def beam_select(logits: Tensor, scores: Tensor, beam: int, termination_symbol: i
         _lib.call("frnnt_beam_select", code, logits.data_ptr(), sb, sk, scores.data_ptr(),
                   None if finished is None else finished.data_ptr(), termination_symbol,
                   best.data_ptr(), parents.data_ptr(), tokens.data_ptr(), scratch.data_ptr(), B, K, V,
-                  beam, _lib.stream_ptr(dev))
+                  beam, _lib.raw_stream(dev.index))
     return best, parents, tokens
 
 
@@ -92,7 +93,9 @@ def beam_reorder(states: Union[Tensor, Sequence[Tensor]], parents: Tensor) -> Un
     if not tensors:
         return []
     assert tensors[0].ndim >= 2 and tensors[0].shape[1] >= 1, tensors[0].shape
-    K, grad = tensors[0].shape[1], torch.is_grad_enabled()
+    K, index = tensors[0].shape[1], dev.index
+    grad, dual = torch.is_grad_enabled(), _lib.tangents_possible()
+    empty_like, contiguous = torch.empty_like, torch.contiguous_format
     rows, out = [], []   # rows: from, to, batch and beam strides, bytes of every tensor
     held = []            # copies stay until the launch
     shape = dtype = None
@@ -103,10 +106,10 @@ def beam_reorder(states: Union[Tensor, Sequence[Tensor]], parents: Tensor) -> Un
                 assert len(shape) >= 2 and shape[0] == B and shape[1] == K, (shape, parents.shape, K)
                 size, complex_ = t.element_size(), t.is_complex()
                 bytes_ = size * math.prod(shape[2:])
-            assert t.device == dev, (t.device, dev)
+            assert t.get_device() == index, (t.device, dev)
             assert not (grad and t.requires_grad), \
                 "beam_reorder has no gradients: call it under torch.no_grad()"
-            assert not _lib.has_tangent(t), "beam_reorder has no forward-mode derivative"
+            assert not (dual and _lib.has_tangent(t)), "beam_reorder has no forward-mode derivative"
             if t.is_neg() or (complex_ and t.is_conj()):   # memory that holds something else
                 t = t.resolve_conj().resolve_neg()
                 held.append(t)
@@ -116,10 +119,9 @@ def beam_reorder(states: Union[Tensor, Sequence[Tensor]], parents: Tensor) -> Un
                     t = t.contiguous()
                 pitch, step = size * t.stride(0), size * t.stride(1)
                 held.append(t)
-            new = (torch.empty_like(t, memory_format=torch.contiguous_format) if k == K
-                   else t.new_empty((B, k) + shape[2:]))
+            new = empty_like(t, memory_format=contiguous) if k == K else t.new_empty((B, k) + shape[2:])
             out.append(new)
             rows += (t.data_ptr(), new.data_ptr(), pitch, step, bytes_)
         _lib.call("frnnt_beam_reorder", len(out), (_c_longlong * len(rows))(*rows), parents.data_ptr(), B, k, K,
-                  _lib.stream_ptr(dev))
+                  _lib.raw_stream(index))
     return out[0] if one else out

@@ -130,7 +130,7 @@ def gated_recurrence(x: Tensor, gate: Tensor, initial: Optional[Tensor] = None,
     x, gate = _rows(x), _rows(gate)
     if (torch.is_grad_enabled() and (x.requires_grad or gate.requires_grad or
                                      (initial is not None and initial.requires_grad))
-            or _lib.has_tangent(x, gate, initial)):   # the autograd function refuses tangents
+            or (_lib.tangents_possible() and _lib.has_tangent(x, gate, initial))):   # the autograd function refuses tangents
         return _GatedRecurrence.apply(x, gate, initial, lengths)
     return _forward(x, gate, initial, lengths, False)[:2]
 
@@ -150,9 +150,11 @@ def gated_recurrence_step(x: Tensor, gate: Tensor, state: Tensor,
     Not differentiable: gated_recurrence is for training.  No counterpart in the reference."""
     assert x.ndim >= 1 and gate.shape == x.shape, (gate.shape, x.shape)
     assert gate.dtype == x.dtype, (gate.dtype, x.dtype)
-    code, kind = _code(x.dtype), _state_type(x.dtype)
+    code = _code(x.dtype)
+    kind = torch.float64 if code == _lib.F64 else torch.float32
     assert state.dtype == kind, (state.dtype, kind)
-    D = x.shape[-1]
+    D, dev = x.shape[-1], x.device
+    index = dev.index
     if parents is None:
         assert state.shape == x.shape, (state.shape, x.shape)
         beams = K = 1
@@ -162,19 +164,19 @@ def gated_recurrence_step(x: Tensor, gate: Tensor, state: Tensor,
         assert parents.shape == x.shape[:2], (parents.shape, x.shape)
         assert parents.dtype == torch.int64, parents.dtype
         assert state.shape == (x.shape[0], K, D), (state.shape, x.shape)
-        assert parents.device == x.device, (parents.device, x.device)
+        assert parents.get_device() == (-1 if index is None else index), (parents.device, dev)
         parents = parents.contiguous()
-    dev = x.device
-    assert x.is_cuda and gate.device == dev and state.device == dev, (dev, gate.device, state.device)
+    assert x.is_cuda and gate.get_device() == index and state.get_device() == index, (dev, gate.device, state.device)
     assert not (torch.is_grad_enabled() and (x.requires_grad or gate.requires_grad or
                                              state.requires_grad)), \
         "gated_recurrence_step has no gradients: use gated_recurrence, or torch.no_grad()"
-    assert not _lib.has_tangent(x, gate, state), "gated_recurrence_step has no forward-mode derivative"
-    x, gate = _lib.plain(x), _lib.plain(gate)
+    assert not (_lib.tangents_possible() and _lib.has_tangent(x, gate, state)), "gated_recurrence_step has no forward-mode derivative"
+    if x.is_neg() or gate.is_neg() or state.is_neg():
+        x, gate, state = x.resolve_neg(), gate.resolve_neg(), state.resolve_neg()
     # rows at one distance from the next
     x2 = x if x.is_contiguous() else _rows(x.reshape(-1, D))
     gate2 = gate if gate.is_contiguous() else _rows(gate.reshape(-1, D))
-    state = _lib.plain(state).contiguous()
+    state = state.contiguous()
     rows = x.numel() // D if D > 0 else 0
     with _lib.on_device(dev):
         new = torch.empty_like(x, dtype=kind, memory_format=torch.contiguous_format)
@@ -184,5 +186,5 @@ def gated_recurrence_step(x: Tensor, gate: Tensor, state: Tensor,
                       gate2.data_ptr(), D if gate2 is gate else gate2.stride(0), state.data_ptr(),
                       None if parents is None else parents.data_ptr(),
                       None if h is new else h.data_ptr(), new.data_ptr(), rows, beams, K, D,
-                      _lib.stream_ptr(dev))
+                      _lib.raw_stream(index))
     return h, new
