@@ -167,16 +167,17 @@ __device__ __forceinline__ void send_pair(uint32_t to, double a, double b, uint3
                : "memory");
 }
 __device__ __forceinline__ bool mail_wait(uint32_t bar, int parity, int tries) {
-  for (int i = 0; i < tries; ++i) {
+  bool arrived = false;
+  for (int i = 0; !arrived && i < tries; ++i) {
     uint32_t done;
     asm volatile("{\n.reg .pred q;\nmbarrier.try_wait.parity.shared::cta.b64 q, [%1], %2;\n"
                  "selp.u32 %0, 1, 0, q;\n}"
                  : "=r"(done)
                  : "r"(bar), "r"(parity)
                  : "memory");
-    if (done != 0) return true;
+    arrived = done != 0;
   }
-  return false;
+  return arrived;
 }
 __device__ __forceinline__ void mail_expect(uint32_t bar, int bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
@@ -191,7 +192,7 @@ __device__ __forceinline__ void mail_begin(const RecMail &mail) {
   if (threadIdx.x < kRecMostCluster) mail.stops[threadIdx.x] = INT_MAX;
   cooperative_groups::this_cluster().sync();   // all have started, and have their mbarriers
 }
-// A turn begins.  Waits run out between the two barriers of a turn: here all threads see the same.
+// Before a turn's first barrier: waits run out between its two, so that all threads see the same here.
 __device__ __forceinline__ void mail_turn(RecMail &mail) { mail.failed = *(volatile int *)mail.gave_up != 0; }
 // Nobody leaves before all that was sent to it has arrived.  A CTA that received every turn has seen
 // that.  One that gave up in turn n has everything up to turn n - 1, and nobody sends it turn n + 2
@@ -298,7 +299,6 @@ recurrence_forward_kernel(RecTensor x, RecTensor gate, const typename S::real *_
   fetch(0);
   if constexpr (CLUSTER) mail_begin(mail);
   for (int turn = 0; turn < turns; ++turn) {
-    if constexpr (CLUSTER) mail_turn(mail);
     fetch(turn + 1);
     copy_wait<1>();
     const int chunk = turn * ranks + rank, first = chunk * kRecChunk + piece_first;
@@ -323,6 +323,7 @@ recurrence_forward_kernel(RecTensor x, RecTensor gate, const typename S::real *_
     }
     put<real, VEC>(EA + S::at(at.piece, at.c), A);
     put<real, VEC>(EB + S::at(at.piece, at.c), B);
+    if constexpr (CLUSTER) mail_turn(mail);
     __syncthreads();
     // join: kRun pieces a thread, then the runs of a channel by shuffles
     real ra[S::kRun], rb[S::kRun], a = real(1), bb = real(0);
@@ -437,7 +438,6 @@ recurrence_backward_kernel(RecTensor x, RecTensor gate, const int64_t *__restric
   fetch(turns - 1);
   if constexpr (CLUSTER) mail_begin(mail);
   for (int turn = turns - 1; turn >= 0; --turn) {
-    if constexpr (CLUSTER) mail_turn(mail);
     if constexpr (!CLUSTER) fetch(turn - 1);
     const int chunk = turn * ranks + rank, first = chunk * kRecChunk + piece_first;
     real start = real(0);   // the state before the tile
@@ -474,6 +474,7 @@ recurrence_backward_kernel(RecTensor x, RecTensor gate, const int64_t *__restric
     put<real, VEC>(EA + S::at(at.piece, at.c), A);
     put<real, VEC>(EB + S::at(at.piece, at.c), B);
     put<real, VEC>(EM + S::at(at.piece, at.c), M);
+    if constexpr (CLUSTER) mail_turn(mail);
     __syncthreads();
     real ra[S::kRun], rb[S::kRun], rm[S::kRun], a = real(1), bb = real(0), m = real(0);
     if (at.joiner) {
