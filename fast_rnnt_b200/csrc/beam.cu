@@ -32,8 +32,8 @@ namespace frnnt {
 
 // Small CTAs, many of them: a row's short phases after the stream run beside other rows' streams
 // (96 x 16 x 31999 fp16: 35 us; 12 CTAs a multiprocessor, with too few registers for that, 40, 256
-// threads and 5 CTAs 39, 64 threads and 24 CTAs 48; reading the same bytes for their maxima
-// alone takes 21 to 24).
+// threads and 5 CTAs 39, 64 threads and 24 CTAs 48; the same loads for their maxima alone take 21
+// to 24).  Chosen on that size only.
 constexpr int kSelThreads = 128, kSelResident = 10;
 constexpr int kSelWarps = kSelThreads / 32;
 constexpr int kSelBeams = 1024;   // most rows of logits of one utterance

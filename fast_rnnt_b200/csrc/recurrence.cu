@@ -15,7 +15,7 @@
 // 5 values an element move instead of 6, and h keeps its 32 bits.
 //
 // Both are bound by memory where there are channels enough: 3 values an element forward, 5
-// backward, in their own type (64 x 500 x 2048 bf16, ragged: 67 and 115 us, 0.9 of the copy rate
+// backward, in their own type (64 x 500 x 2048 bf16, ragged: 65 and 113 us, 0.9 of the copy rate
 // if nothing were padding).  Inputs go to shared memory with cp.async a tile ahead, each thread
 // fetching just what it reads itself, so that no barrier belongs to the copies.  Tiles of 32
 // channels and 128 threads, four CTAs a multiprocessor forward and three backward, took the place

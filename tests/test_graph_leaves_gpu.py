@@ -166,3 +166,23 @@ def test_part_of_a_leaf_as_an_input_of_its_own():
     torch.cuda.synchronize()
     want = torch.cat(plain_gradients(x, gate), -1) + 1
     assert torch.equal(both.grad, want)
+
+
+def test_second_capture_of_the_same_leaves():
+    """The first one's loss holds their accumulators, on the stream of the captures."""
+    from fast_rnnt_b200.graphs import GraphedStep
+    x, gate = (t.requires_grad_(True) for t in make(10))
+
+    def step(t):
+        loss = loss_of(t["x"], t["gate"])
+        loss.backward()
+        return loss
+
+    first = GraphedStep(step, dict(x=x, gate=gate))
+    second = GraphedStep(step, dict(x=x, gate=gate))
+    batch = make(11)
+    replayed(second, (x, gate), batch)
+    assert all(torch.equal(t.grad, w) for t, w in zip((x, gate), plain_gradients(*batch)))
+    first()
+    torch.cuda.synchronize()
+    assert torch.equal(first.loss, second.loss)
